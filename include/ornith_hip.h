@@ -420,6 +420,104 @@ ORNITH_API int ornith_sdpa_prefill_gated(ornith_ctx* ctx, const void* d_q_rot, c
                                          const void* d_v_cache, const void* d_qg, int T, int Hq, int Hkv,
                                          int hd, int offset, int cap, float scale, void* d_out);
 
+/* ---- several continuations of one prompt: a paged KV cache ------------------------
+ * No counterpart in the reference, which serves one sequence from one contiguous cache
+ * (src/model/cache.rs:38-79). A sequence's rows lie on pages: row j on page table[j / page_rows],
+ * row j % page_rows of it. Sequences that share a prefix share its pages. The descriptor holds
+ * every full-attention layer's pages; its two arrays of pointers are host memory and are read
+ * during a call only. */
+typedef struct ornith_kv_pages {
+  int n_layers;
+  int n_pages;
+  int page_rows;    /* a power of two, 16 .. 256 */
+  int Hkv, hd;      /* hd: 64, 128 or 256 */
+  void* const* d_k; /* n_layers device pointers (16-byte aligned): bf16 [n_pages, Hkv, page_rows, hd] */
+  void* const* d_v;
+} ornith_kv_pages;
+/* The sequences of one call. The tables and lengths live on the device and cannot be validated
+ * here: a length is taken as 0 below 0 and as max_rows above it; a read through a page id past
+ * the end reads the last page, a write through one is dropped. */
+typedef struct ornith_kv_batch {
+  int B;                   /* sequences, 1 .. 4096 */
+  int table_stride;        /* entries a sequence has in d_table */
+  const uint32_t* d_table; /* [B, table_stride] page ids */
+  const int32_t* d_lens;   /* [B] rows held, those of the call itself included */
+  int shared_rows;         /* the first shared_rows rows (whole pages) are the same pages for all B:
+                              they are read once for all, through the first sequence's table */
+  int max_rows;            /* no sequence holds more */
+} ornith_kv_batch;
+
+/* Page dst[i] := page src[i], the first `rows` rows of every head, in all layers; host id lists,
+ * n >= 0 pairs, which the caller may reuse at once. One source may have several destinations; a
+ * page written twice, or both read and written, is refused. */
+ORNITH_API int ornith_kv_pages_copy(ornith_ctx* ctx, const ornith_kv_pages* pages, const uint32_t* src, const uint32_t* dst, int n,
+                                    int rows);
+/* Rows [row0, row0 + rows) of one layer's contiguous caches (bf16 [Hkv, cap, hd], as
+ * ornith_attn_prep fills them) into rows [at, at + rows) of the sequence whose pages the host list
+ * ids[0 .. n_ids) names, and back. Only the pages of those rows are looked at. */
+ORNITH_API int ornith_kv_pages_load(ornith_ctx* ctx, const ornith_kv_pages* pages, int layer, const void* d_k_cache,
+                                    const void* d_v_cache, int cap, int row0, int rows, const uint32_t* ids, int n_ids, int at);
+ORNITH_API int ornith_kv_pages_store(ornith_ctx* ctx, const ornith_kv_pages* pages, int layer, void* d_k_cache, void* d_v_cache, int cap,
+                                     int row0, int rows, const uint32_t* ids, int n_ids, int at);
+
+/* ornith_attn_prep for a batch: T new rows (1 .. 64) of every sequence, row t of sequence b at
+ * position d_lens[b] - T + t (a row of negative position, in a sequence shorter than T, is left
+ * out). qg [B, T, Hq, 2*hd], kx / vx [B, T, Hkv, hd]; q_rot [B, T, Hq, hd] receives the rotated
+ * queries, the pages the new K and V rows. The norm and the rotation are rounded to bf16 once, at
+ * the end, where ornith_attn_prep also rounds inside the norm: the two agree to rounding.
+ * rope_dims a multiple of hd / 32, halves rotate against each other; table_npos >= max_rows. Two
+ * sequences of a batch must not append to the same page. */
+ORNITH_API int ornith_attn_prep_paged(ornith_ctx* ctx, const ornith_kv_pages* pages, int layer, const ornith_kv_batch* batch,
+                                      const void* d_qg, const void* d_kx, const void* d_vx, const void* d_q_norm_w,
+                                      const void* d_k_norm_w, int T, int Hq, int rope_dims, float eps, const float* d_cos,
+                                      const float* d_sin, int table_npos, void* d_q_rot);
+/* ornith_sdpa_decode_gated for a batch over pages: row t of sequence b sees the keys
+ * [0, d_lens[b] - T + t]; a row that sees none gives zeros. out bf16 [B, T, Hq, hd] =
+ * sigmoid(gate) * attention, gate in the second half of d_qg [B, T, Hq, 2*hd]; with d_qg null the
+ * attention alone. scale > 0. Scores, softmax and sums are fp32, probabilities go to the matrix
+ * cores as bf16: the results agree with ornith_sdpa_decode_gated's to rounding, not bit for bit. */
+ORNITH_API int ornith_sdpa_paged_gated(ornith_ctx* ctx, const ornith_kv_pages* pages, int layer, const ornith_kv_batch* batch,
+                                       const void* d_q_rot, const void* d_qg, int T, int Hq, float scale, void* d_out);
+
+/* A pool that owns such pages and knows which sequence holds which: bookkeeping on the host, page
+ * copies on the context's stream. Sequences are small numbers below max_seqs. A call that fails
+ * changes nothing. */
+typedef struct ornith_kv_pool ornith_kv_pool;
+/* max_pages: pages one sequence may hold */
+ORNITH_API int ornith_kv_pool_create(ornith_ctx* ctx, int n_layers, int n_pages, int page_rows, int Hkv, int hd, int max_seqs,
+                                     int max_pages, ornith_kv_pool** out);
+ORNITH_API int ornith_kv_pool_destroy(ornith_kv_pool* pool);
+/* the pool's pages (valid while it lives) */
+ORNITH_API int ornith_kv_pool_pages(const ornith_kv_pool* pool, ornith_kv_pages* out);
+/* an empty sequence; the lowest free number */
+ORNITH_API int ornith_kv_pool_open(ornith_kv_pool* pool, int* seq_out);
+/* n more sequences with the same rows: all pages are shared, and the one that is not full is copied
+ * by whoever extends it first */
+ORNITH_API int ornith_kv_pool_fork(ornith_kv_pool* pool, int seq, int n, int* seqs_out);
+/* `rows` more rows for each of n different sequences: pages are taken (lowest id first), shared
+ * pages that will be written are copied. What the new rows hold is undefined until written. */
+ORNITH_API int ornith_kv_pool_extend(ornith_kv_pool* pool, const int* seqs, int n, int rows);
+/* keep the first `rows` rows (a rejected draft, a rewind); pages behind them are given back */
+ORNITH_API int ornith_kv_pool_truncate(ornith_kv_pool* pool, int seq, int rows);
+ORNITH_API int ornith_kv_pool_close(ornith_kv_pool* pool, int seq);
+/* Used pages to the lowest ids; *moved (may be null) = pages copied. Page ids read before change. */
+ORNITH_API int ornith_kv_pool_compact(ornith_kv_pool* pool, int* moved);
+/* rows a sequence holds, and its page ids: with ids_out == NULL only their number */
+ORNITH_API int ornith_kv_pool_seq(const ornith_kv_pool* pool, int seq, int* rows_out, uint32_t* ids_out, int cap, int* n_ids_out);
+ORNITH_API int ornith_kv_pool_stats(const ornith_kv_pool* pool, int* pages_used, int* pages_shared, int* seqs_open);
+/* Rows [row0, row0 + rows) of contiguous caches as rows [at, ..) of a sequence that holds them
+ * (ornith_kv_pool_extend first), and back. A load refuses rows on a page that another sequence
+ * shares. */
+ORNITH_API int ornith_kv_pool_load(ornith_kv_pool* pool, int seq, int layer, const void* d_k_cache, const void* d_v_cache, int cap,
+                                   int row0, int rows, int at);
+ORNITH_API int ornith_kv_pool_store(ornith_kv_pool* pool, int seq, int layer, void* d_k_cache, void* d_v_cache, int cap, int row0,
+                                    int rows, int at);
+/* The descriptor of a batch of n different sequences, for the calls above: tables and lengths in
+ * the pool's own device memory, shared_rows the full pages that all of them share. It holds until
+ * the next ornith_kv_pool_batch, or until a sequence of it is extended, truncated, closed or moved by
+ * a compaction. */
+ORNITH_API int ornith_kv_pool_batch(ornith_kv_pool* pool, const int* seqs, int n, ornith_kv_batch* out);
+
 /* ---- greedy selection: src/ops/sample.rs ------------------------------------------ */
 /* greedy_token / the verify rows of generate_step_mtp (src/ops/sample.rs:134-147,
  * src/mtp_generate.rs:237-250): tokens[r] = argmax_i bf16(logits[r,i] - lse_r), lowest
@@ -439,6 +537,21 @@ ORNITH_API int ornith_greedy_rows_noalloc(ornith_ctx* ctx, const void* d_logits,
  * chain's choice. */
 ORNITH_API int ornith_argmax_rows(ornith_ctx* ctx, const void* d_logits, int rows, int V,
                                   uint32_t* d_out);
+
+/* Log probabilities of given tokens under rows of logits (bf16 or f32 by dtype, row r at
+ * d_logits + r * row_stride elements, no alignment beyond the element's), for scoring a text or
+ * ranking continuations; no counterpart in the reference. Natural logarithms, all outputs fp32:
+ *   d_logprobs [rows, n_tokens]  of d_tokens [rows, n_tokens]; n_tokens may be 0 (both may be null)
+ *   d_entropy, d_lse [rows]      may be null
+ *   d_top_ids, d_top_logprobs [rows, k]  the k <= 32 most probable tokens, falling; equal logits by
+ *                                the lower id; k may be 0 (both may be null)
+ * A logit of -inf (a masked token) has probability 0 and log probability -inf; so has a token id
+ * past the end. A row of nothing but -inf has lse -inf and entropy 0. A row with a NaN or +inf
+ * logit has no distribution: its lse, entropy and the log probabilities of its finite tokens are
+ * not numbers (or -inf); the alternatives' ids still go by value, NaN last. */
+ORNITH_API int ornith_token_logprobs(ornith_ctx* ctx, const void* d_logits, int dtype, int rows, int V, int64_t row_stride,
+                                     const uint32_t* d_tokens, int n_tokens, int k, float* d_logprobs, float* d_entropy, float* d_lse,
+                                     uint32_t* d_top_ids, float* d_top_logprobs);
 
 /* ---- weights: WeightStore (src/weights.rs:41-279) -------------------------------
  * A named-tensor store on the device. Names are the reference's

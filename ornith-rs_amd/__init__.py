@@ -384,6 +384,71 @@ def attn_decode(self, qg, kx, vx, qw, kw, T, Hq, Hkv, hd, rope_dims, eps, cos_t,
                                     q_rot.ptr, k_cache.ptr, v_cache.ptr, out.ptr), "attn_decode")
 
 
+# ---- paged KV caches: several continuations of one prompt ------------------------------
+class KvPagesStruct(C.Structure):
+    _fields_ = [("n_layers", C.c_int), ("n_pages", C.c_int), ("page_rows", C.c_int), ("Hkv", C.c_int), ("hd", C.c_int),
+                ("d_k", C.POINTER(C.c_void_p)), ("d_v", C.POINTER(C.c_void_p))]
+
+
+class KvBatchStruct(C.Structure):
+    _fields_ = [("B", C.c_int), ("table_stride", C.c_int), ("d_table", C.c_void_p), ("d_lens", C.c_void_p), ("shared_rows", C.c_int),
+                ("max_rows", C.c_int)]
+
+
+class KvPages:
+    """Pages of a KV cache: k, v lists of one buffer a layer, bf16 [n_pages, Hkv, page_rows, hd]."""
+
+    def __init__(self, k, v, n_pages, page_rows, Hkv, hd):
+        assert len(k) == len(v), (len(k), len(v))
+        self.keep = (k, v, (C.c_void_p * len(k))(*[b.ptr for b in k]), (C.c_void_p * len(v))(*[b.ptr for b in v]))
+        self.s = KvPagesStruct(len(k), n_pages, page_rows, Hkv, hd, self.keep[2], self.keep[3])
+
+
+class KvBatch:
+    """Sequences of a call: table u32 [B, table_stride], lens i32 [B] (device); ornith_kv_batch."""
+
+    def __init__(self, B, table, table_stride, lens, shared_rows, max_rows):
+        self.keep = (table, lens)
+        self.s = KvBatchStruct(B, table_stride, table.ptr if table else None, lens.ptr if lens else None, shared_rows, max_rows)
+
+
+def _ids(a):
+    return np.ascontiguousarray(a, dtype=np.uint32)
+
+
+@_ctx_method
+def kv_pages_copy(self, pages, src, dst, rows):
+    src, dst = _ids(src), _ids(dst)
+    assert src.size == dst.size, (src.size, dst.size)
+    _check(lib().ornith_kv_pages_copy(self.h, C.byref(pages.s), _ptr(src), _ptr(dst), src.size, rows), "kv_pages_copy")
+
+
+@_ctx_method
+def kv_pages_load(self, pages, layer, k_cache, v_cache, cap, row0, rows, ids, at):
+    ids = _ids(ids)
+    _check(lib().ornith_kv_pages_load(self.h, C.byref(pages.s), layer, k_cache.ptr, v_cache.ptr, cap, row0, rows, _ptr(ids), ids.size, at),
+           "kv_pages_load")
+
+
+@_ctx_method
+def kv_pages_store(self, pages, layer, k_cache, v_cache, cap, row0, rows, ids, at):
+    ids = _ids(ids)
+    _check(lib().ornith_kv_pages_store(self.h, C.byref(pages.s), layer, k_cache.ptr, v_cache.ptr, cap, row0, rows, _ptr(ids), ids.size, at),
+           "kv_pages_store")
+
+
+@_ctx_method
+def attn_prep_paged(self, pages, layer, batch, qg, kx, vx, qw, kw, T, Hq, rope_dims, eps, cos_t, sin_t, npos, q_rot):
+    _check(lib().ornith_attn_prep_paged(self.h, C.byref(pages.s), layer, C.byref(batch.s), qg.ptr, kx.ptr, vx.ptr, qw.ptr, kw.ptr, T, Hq,
+                                        rope_dims, C.c_float(eps), cos_t.ptr, sin_t.ptr, npos, q_rot.ptr), "attn_prep_paged")
+
+
+@_ctx_method
+def sdpa_paged_gated(self, pages, layer, batch, q_rot, qg, T, Hq, scale, out):
+    _check(lib().ornith_sdpa_paged_gated(self.h, C.byref(pages.s), layer, C.byref(batch.s), q_rot.ptr, qg.ptr if qg else None, T, Hq,
+                                         C.c_float(scale), out.ptr), "sdpa_paged_gated")
+
+
 # ---- greedy selection ----------------------------------------------------------------
 @_ctx_method
 def greedy_rows(self, logits, rows, V, tokens, lse=None):
@@ -403,5 +468,16 @@ def argmax_rows(self, logits, rows, V, out):
     _check(lib().ornith_argmax_rows(self.h, logits.ptr, rows, V, out.ptr), "argmax_rows")
 
 
+# ---- scores --------------------------------------------------------------------------
+@_ctx_method
+def token_logprobs(self, logits, dtype, rows, V, tokens, n_tokens, k, logprobs, entropy=None, lse=None, top_ids=None, top_logprobs=None,
+                   row_stride=None):
+    """ornith_token_logprobs: given tokens' log probabilities, entropy, logsumexp and the k best alternatives."""
+    _check(lib().ornith_token_logprobs(self.h, logits.ptr, dtype, rows, V, C.c_int64(V if row_stride is None else row_stride),
+                                       tokens.ptr if tokens else None, n_tokens, k, logprobs.ptr if logprobs else None,
+                                       entropy.ptr if entropy else None, lse.ptr if lse else None, top_ids.ptr if top_ids else None,
+                                       top_logprobs.ptr if top_logprobs else None), "token_logprobs")
+
+
 from .engine import *  # noqa: E402,F401,F403  (engine objects: WeightStore, TextModel, ...)
-from .engine import TextConfig, Sampler, MtpStats, WeightStore, Caches, TextModel, FrSpec, MtpHead, generate_step, generate_step_mtp, HISTORY_CYCLE, HISTORY_COMMITTED  # noqa: E402,F401
+from .engine import KvPool, TextConfig, Sampler, MtpStats, WeightStore, Caches, TextModel, FrSpec, MtpHead, generate_step, generate_step_mtp, HISTORY_CYCLE, HISTORY_COMMITTED  # noqa: E402,F401

@@ -85,6 +85,23 @@ int ornith_greedy_rows_ws(ornith_ctx* ctx, const void* d_logits, int rows, int V
 // (which must be current) once per device; ornith_ctx_create keeps it in the context.
 int ornith_sample_init_device(int device, void** ptr_out);
 
+// The context's device is the current one while this lives: a launch goes to it whatever device the
+// calling thread had selected, and the thread finds its own again afterwards.
+class OrnDevice {
+ public:
+  explicit OrnDevice(const ornith_ctx* ctx) : want_(ctx->device), had_(ctx->device) {
+    if (hipGetDevice(&had_) == hipSuccess && had_ != want_) (void)hipSetDevice(want_);
+  }
+  ~OrnDevice() {
+    if (had_ != want_) (void)hipSetDevice(had_);
+  }
+  OrnDevice(const OrnDevice&) = delete;
+  OrnDevice& operator=(const OrnDevice&) = delete;
+
+ private:
+  int want_, had_;
+};
+
 // Records the message for ornith_last_error() and returns `code`.
 int ornith_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 

@@ -7,7 +7,7 @@ import os
 
 import numpy as np
 
-from . import (BF16, F32, LinearStruct, OrnithError, _check, _ptr, lib)
+from . import (BF16, F32, KvBatch, KvBatchStruct, KvPages, KvPagesStruct, LinearStruct, OrnithError, _check, _ptr, lib)
 
 DT_F32, DT_BF16, DT_F16, DT_U8, DT_U32, DT_I32 = range(6)
 DT_I8, DT_I16, DT_U16, DT_I64, DT_U64, DT_F64, DT_BOOL = range(6, 13)
@@ -626,3 +626,71 @@ def moe_close(ctx, w, res, y, wnorm, wnext, eps, T, h, normed, out, x_out, next_
 def add_rms_moe_block(ctx, w, res, y, wnorm, eps, T, h_out, normed_out, out):
     _check(lib().ornith_add_rms_moe_block(ctx.h, C.byref(w), res.ptr, y.ptr, wnorm.ptr, C.c_float(eps), T,
                                           h_out.ptr, normed_out.ptr, out.ptr), "add_rms_moe_block")
+
+
+class KvPool:
+    """ornith_kv_pool: pages of a KV cache and the sequences that hold them. Sequences are small ints."""
+
+    def __init__(self, ctx, n_layers, n_pages, page_rows, Hkv, hd, max_seqs, max_pages):
+        self.ctx, h = ctx, C.c_void_p()
+        _check(lib().ornith_kv_pool_create(ctx.h, n_layers, n_pages, page_rows, Hkv, hd, max_seqs, max_pages, C.byref(h)), "kv_pool_create")
+        self.h, self.page_rows = h, page_rows
+        self.pages = KvPages.__new__(KvPages)
+        self.pages.s = KvPagesStruct()
+        _check(lib().ornith_kv_pool_pages(h, C.byref(self.pages.s)), "kv_pool_pages")
+
+    def close(self):
+        if self.h:
+            lib().ornith_kv_pool_destroy(self.h)
+            self.h = None
+
+    def open(self):
+        s = C.c_int()
+        _check(lib().ornith_kv_pool_open(self.h, C.byref(s)), "kv_pool_open")
+        return s.value
+
+    def fork(self, seq, n):
+        out = (C.c_int * max(n, 1))()
+        _check(lib().ornith_kv_pool_fork(self.h, seq, n, out), "kv_pool_fork")
+        return list(out)
+
+    def extend(self, seqs, rows):
+        _check(lib().ornith_kv_pool_extend(self.h, (C.c_int * len(seqs))(*seqs), len(seqs), rows), "kv_pool_extend")
+
+    def truncate(self, seq, rows):
+        _check(lib().ornith_kv_pool_truncate(self.h, seq, rows), "kv_pool_truncate")
+
+    def close_seq(self, seq):
+        _check(lib().ornith_kv_pool_close(self.h, seq), "kv_pool_close")
+
+    def compact(self):
+        n = C.c_int()
+        _check(lib().ornith_kv_pool_compact(self.h, C.byref(n)), "kv_pool_compact")
+        return n.value
+
+    def seq(self, seq):
+        """(rows, page ids) of a sequence."""
+        rows, n = C.c_int(), C.c_int()
+        _check(lib().ornith_kv_pool_seq(self.h, seq, C.byref(rows), None, 0, C.byref(n)), "kv_pool_seq")
+        ids = np.empty(n.value, np.uint32)
+        _check(lib().ornith_kv_pool_seq(self.h, seq, None, _ptr(ids), n.value, None), "kv_pool_seq")
+        return rows.value, ids
+
+    def stats(self):
+        """(pages used, pages shared, sequences open)"""
+        v = [C.c_int() for _ in range(3)]
+        _check(lib().ornith_kv_pool_stats(self.h, *[C.byref(x) for x in v]), "kv_pool_stats")
+        return tuple(x.value for x in v)
+
+    def load(self, seq, layer, k_cache, v_cache, cap, row0, rows, at):
+        _check(lib().ornith_kv_pool_load(self.h, seq, layer, k_cache.ptr, v_cache.ptr, cap, row0, rows, at), "kv_pool_load")
+
+    def store(self, seq, layer, k_cache, v_cache, cap, row0, rows, at):
+        _check(lib().ornith_kv_pool_store(self.h, seq, layer, k_cache.ptr, v_cache.ptr, cap, row0, rows, at), "kv_pool_store")
+
+    def batch(self, seqs):
+        """The descriptor of these sequences for attn_prep_paged / sdpa_paged_gated (see ornith_kv_pool_batch)."""
+        b = KvBatch.__new__(KvBatch)
+        b.s = KvBatchStruct()
+        _check(lib().ornith_kv_pool_batch(self.h, (C.c_int * len(seqs))(*seqs), len(seqs), C.byref(b.s)), "kv_pool_batch")
+        return b
