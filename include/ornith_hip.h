@@ -546,7 +546,7 @@ ORNITH_API int ornith_argmax_rows(ornith_ctx* ctx, const void* d_logits, int row
  *   d_top_ids, d_top_logprobs [rows, k]  the k <= 32 most probable tokens, falling; equal logits by
  *                                the lower id; k may be 0 (both may be null)
  * A logit of -inf (a masked token) has probability 0 and log probability -inf; so has a token id
- * past the end. At most 65535 rows a call. A row of nothing but -inf has lse -inf and entropy 0. A row with a NaN or +inf
+ * past the end. At most 65535 rows of 2097148 logits a call. A row of nothing but -inf has lse -inf and entropy 0. A row with a NaN or +inf
  * logit has no distribution: its lse, entropy and the log probabilities of its finite tokens are
  * not numbers (or -inf); the alternatives' ids still go by value, NaN last. */
 ORNITH_API int ornith_token_logprobs(ornith_ctx* ctx, const void* d_logits, int dtype, int rows, int V, int64_t row_stride,

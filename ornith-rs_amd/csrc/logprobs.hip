@@ -19,10 +19,16 @@ constexpr int kMaxTop = 32;  // alternatives a row
 // wavefront takes some groups one after another and leaves its (m, L, S) and every group's best value.
 // The second, a workgroup a row, joins the sums; and as the k best tokens of a row lie in its k best
 // groups (by best value, then by place: each of k better groups holds a token that comes before any of
-// the group's), it looks through those alone.
-constexpr int kGroups = 512;                 // groups a row at most
-constexpr int kCands = 512;                  // candidates that are ranked against each other
+// the group's), it looks through those alone, and in them, for the same reason, at the k best 16-byte
+// pieces.
 constexpr int kFinish = 1024;                // threads of the second launch
+constexpr int kPass = 4;                     // passes of so many threads over a row's groups, or over the pieces of the best ones
+constexpr int kGroups = kPass * kFinish;     // groups a row at most
+constexpr int kGroupPieces = 128;            // 16-byte pieces a group: 2 KB, two loads a lane
+static_assert(kMaxTop * kGroupPieces <= kPass * kFinish, "the best groups' pieces in as many passes");
+constexpr int kCands = 256;                  // candidates that are ranked against each other
+static_assert(kMaxTop * 8 <= kCands, "the best pieces' tokens among them");
+constexpr int kMaxV = (kGroups * kGroupPieces - 1) * 4;  // logits a row: what fits kGroups groups of fp32 at any alignment
 constexpr float kL2E = 1.44269502162933349609375f, kL2ELow = 1.925963033500e-8f, kLn2 = 0.693147180559945309f;
 constexpr float kFloor = -200.f;             // e^kFloor is 0 in fp32: differences stop there, so that -inf makes no NaN
 
@@ -40,7 +46,7 @@ struct LogprobArgs {
   uint32_t* best;          // [rows, groups]: order of the best value
   int64_t stride;
   int V, n_tokens, k;
-  int steps, groups, run, runs;  // loads a lane a group; groups a row; groups a wavefront takes; wavefronts a row
+  int groups, run, runs;   // groups a row; groups a wavefront takes; wavefronts a row
 };
 
 // A value's place among all: larger for a larger value, -0 and 0 the same, NaN below everything.
@@ -49,26 +55,30 @@ __device__ __forceinline__ uint32_t order_of(float v) {
   return v != v ? 0u : v == 0.f ? 0x80000000u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// A row as 16-byte pieces at 16-byte addresses: piece j holds tokens [PER j - head, + PER); what lies
-// outside the row is not read.
+// A row as 16-byte pieces at 16-byte addresses: piece j holds tokens [PER j - head, + PER). The first
+// piece may begin before the row (in the 16 bytes that hold its first token) and the last end behind
+// it: what is no token of the row is told apart by its number, and nothing behind the piece that
+// holds the last one is read.
 template <bool F32>
 struct Row {
   static constexpr int PER = F32 ? 4 : 8, ES = F32 ? 4 : 2;
   const unsigned char* base;  // of token 0
+  __amdgpu_buffer_rsrc_t buf;
   int V, head;
   __device__ __forceinline__ Row(const LogprobArgs& p, size_t row) {
     base = static_cast<const unsigned char*>(p.x) + (size_t)(row * p.stride) * ES;
     V = p.V;
     head = (int)((uintptr_t)base & 15) / ES;
+    buf = dm_buffer(base - head * ES, ((V + head) * ES + 3) & ~3);
   }
   __device__ __forceinline__ float at(int i) const {
     if constexpr (F32) return reinterpret_cast<const float*>(base)[i];
     return dm_bf2f(reinterpret_cast<const bf16_t*>(base)[i]);
   }
   __device__ __forceinline__ int first(int piece) const { return PER * piece - head; }
-  __device__ __forceinline__ bool inside(int piece) const { return first(piece) >= 0 && first(piece) + PER <= V; }
-  __device__ __forceinline__ u32x4_t raw(int piece) const { return *reinterpret_cast<const u32x4_t*>(base + (ptrdiff_t)ES * first(piece)); }
-  static __device__ __forceinline__ void values(const u32x4_t& w, float (&x)[PER]) {
+  __device__ __forceinline__ bool has(int t) const { return (unsigned)t < (unsigned)V; }
+  __device__ __forceinline__ void load(int piece, float (&x)[PER]) const {
+    const dm_u32x4 w = __builtin_bit_cast(dm_u32x4, __builtin_amdgcn_raw_buffer_load_b128(buf, 16 * piece, 0, 0));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (F32) {
@@ -76,18 +86,6 @@ struct Row {
       } else {
         x[2 * i] = dm_bf2f_lo(w[i]);
         x[2 * i + 1] = dm_bf2f_hi(w[i]);
-      }
-    }
-  }
-  // -inf outside the row
-  __device__ __forceinline__ void load(int piece, float (&x)[PER]) const {
-    if (inside(piece)) {
-      values(raw(piece), x);
-    } else {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int t = first(piece) + i;
-        x[i] = t >= 0 && t < V ? at(t) : -DM_INF;
       }
     }
   }
@@ -114,45 +112,47 @@ __global__ __launch_bounds__(256) void logprobs_sum_kernel(LogprobArgs p) {
   const int g_end = min(p.groups, (w + 1) * p.run);
   float m = -DM_INF, l = 0.f, s = 0.f, c = 0.f;
   for (int g = w * p.run; g < g_end; ++g) {
-    float best = -DM_INF;
-    bool low = false;
-    for (int st = 0; st < p.steps; st += 2) {
-      float x[2][PER];
-      const int piece = (g * p.steps + st) * 64 + lane;
-      r.load(piece, x[0]);
-      r.load(piece + 64, x[1]);
-      float mx = -DM_INF;
+    float x[2][PER];
+    const int piece = g * kGroupPieces + lane;
+    r.load(piece, x[0]);
+    r.load(piece + 64, x[1]);
+    if (r.first(g * kGroupPieces) < 0 || r.first((g + 1) * kGroupPieces) > p.V) {  // the row's first group or its last
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < PER; ++i) mx = fmaxf(mx, x[u][i]);
-      mx = dm_wave_max<64>(mx);
-      if (mx == -DM_INF) {  // masked tokens or NaN only: which of them
+        for (int i = 0; i < PER; ++i) x[u][i] = r.has(r.first(piece + 64 * u) + i) ? x[u][i] : -DM_INF;
+    }
+    float best = -DM_INF;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const int t = r.first(piece + 64 * u) + i;
-            low = low || (t >= 0 && t < p.V && x[u][i] == -DM_INF);
-          }
-      }
-      best = fmaxf(best, mx);
-      if (mx > m) move_to(mx, m, l, s, c);
-      const float ref = m > -DM_INF ? m : 0.f;
+      for (int i = 0; i < PER; ++i) best = fmaxf(best, x[u][i]);
+    best = dm_wave_max<64>(best);
+    bool low = false;
+    if (best == -DM_INF) {  // masked tokens or NaN only: which of them
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          // e^d = 2^t (1 + ln2 (lo + d kL2ELow)): t is rounded at its own size, and what that takes is put
-          // back in the sum (C), or a sure token's probability would carry the error of far smaller ones
-          const float d = __builtin_elementwise_maximum(x[u][i] - ref, kFloor);
-          const float t = d * kL2E, lo = dm_fma(d, kL2E, -t);
-          const float e = __builtin_amdgcn_exp2f(t);
-          l += e;
-          s = dm_fma(e, d, s);
-          c = dm_fma(e, lo, c);
+          const int t = r.first(piece + 64 * u) + i;
+          low = low || (r.has(t) && x[u][i] == -DM_INF);
         }
     }
+    if (best > m) move_to(best, m, l, s, c);
+    const float ref = m > -DM_INF ? m : 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        // e^d = 2^t (1 + ln2 (lo + d kL2ELow)): t is rounded at its own size, and what that takes is put
+        // back in the sum (C), or a sure token's probability would carry the error of far smaller ones
+        const float d = __builtin_elementwise_maximum(x[u][i] - ref, kFloor);
+        const float t = d * kL2E, lo = dm_fma(d, kL2E, -t);
+        const float e = __builtin_amdgcn_exp2f(t);
+        l += e;
+        s = dm_fma(e, d, s);
+        c = dm_fma(e, lo, c);
+      }
     if (p.k) {
       uint32_t o = order_of(best);
       if (best == -DM_INF && __builtin_amdgcn_ballot_w64(low) == 0) o = 0;
@@ -165,54 +165,158 @@ __global__ __launch_bounds__(256) void logprobs_sum_kernel(LogprobArgs p) {
   if (lane == 0) p.sums[row * p.runs + w] = make_float4(m, l, s, c);
 }
 
-__device__ __forceinline__ float wg_sum(float v, float* red) {
-  v = dm_wave_sum<64>(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[threadIdx.x & 15];
-  return dm_row_sum(v);
+// The value that order_of made `o` of (-0 as 0, any NaN as one).
+__device__ __forceinline__ float value_of(uint32_t o) {
+  return o == 0 ? __builtin_nanf("") : __uint_as_float((o & 0x80000000u) ? o ^ 0x80000000u : ~o);
 }
-__device__ __forceinline__ float wg_max(float v, float* red) {
-  v = dm_wave_max<64>(v);
+
+struct Select {
+  uint32_t key[kPass * kFinish];
+  uint32_t range[kFinish / 64][2];
+  uint32_t counts[2][kFinish / 64][2];
+  int list[kMaxTop], found[64], n;
+  uint32_t least;
+};
+
+// the value of lane l ^ S, and what the lanes of a wavefront (W = 64) or of a row of 16 come to
+template <int S>
+__device__ __forceinline__ uint32_t other(uint32_t v) { return __float_as_uint(dm_xor_lane<S>(__uint_as_float(v))); }
+template <int W, class Op>
+__device__ __forceinline__ uint32_t all_lanes(uint32_t v, Op op) {
+  if constexpr (W == 64) {
+    v = op(v, other<32>(v));
+    v = op(v, other<16>(v));
+  }
+  v = op(v, other<8>(v));
+  v = op(v, other<4>(v));
+  v = op(v, other<2>(v));
+  return op(v, other<1>(v));
+}
+
+// The k best of sh.key[0 .. n), n >= k, equal ones by the lower number, their numbers into sh.list, best
+// first; returns the least of them. The workgroup counts, two bits of a bound a turn, how
+// many keys reach it; it starts below what the largest and the smallest have in common and is done as
+// soon as that are no more than a wavefront has lanes: those are ranked. More equal keys than that at the bound are
+// cut the same way by their numbers. (Loops stay loops here: a launch of one workgroup takes as long
+// as its code takes to arrive.)
+__device__ __forceinline__ uint32_t select_best(int n, int k, Select& sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto add = [](uint32_t a, uint32_t b) { return a + b; };
+  auto larger = [](uint32_t a, uint32_t b) { return max(a, b); };
+  uint32_t hi = 0, lo = 0;  // of the keys, and of their complements
+#pragma unroll 1
+  for (int i = tid; i < n; i += kFinish) {
+    hi = max(hi, sh.key[i]);
+    lo = max(lo, ~sh.key[i]);
+  }
+  hi = all_lanes<64>(hi, larger);
+  lo = all_lanes<64>(lo, larger);
+  if (lane == 0) {
+    sh.range[wave][0] = hi;
+    sh.range[wave][1] = lo;
+  }
+  if (tid == 0) sh.n = 0;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  hi = all_lanes<16>(sh.range[lane & 15][0], larger);
+  lo = ~all_lanes<16>(sh.range[lane & 15][1], larger);
+  const uint32_t same = hi ^ lo;
+  int have = n, bit = same ? (31 - __builtin_clz(same)) & ~1 : -2;  // pairs of bits from the one that holds the first difference
+  uint32_t bound = bit < 0 ? lo : bit == 30 ? 0 : hi >> (bit + 2) << (bit + 2), edge = 0;
+  bool by_number = false;
+  auto value = [&](int i) {
+    const uint32_t v = i < n ? sh.key[i] : 0;
+    return !by_number ? v : v > edge ? 0x2000u : v == edge && i < n ? 0x1fffu - i : 0u;
+  };
+  static_assert(kPass * kFinish <= 0x1000, "numbers in twelve bits");
+  int turn = 0;
+#pragma unroll 1
+  for (;;) {
+    if (have <= 64 || bit < 0) {
+      if (have <= 64) break;  // (numbers are all different: cut by them, 64 is reached)
+      by_number = true;
+      edge = bound;
+      bound = 0;
+      bit = 12;
+    }
+    const uint32_t one = bound | 1u << bit, two = bound | 2u << bit, three = bound | 3u << bit;
+    int c1 = 0, c2 = 0, c3 = 0;
+#pragma unroll 1
+    for (int i = wave * 64; i < n; i += kFinish) {
+      const uint32_t v = value(i + lane);
+      c1 += __popcll(__builtin_amdgcn_ballot_w64(v >= one));
+      c2 += __popcll(__builtin_amdgcn_ballot_w64(v >= two));
+      c3 += __popcll(__builtin_amdgcn_ballot_w64(v >= three));
+    }
+    if (lane == 0) {
+      sh.counts[turn][wave][0] = (uint32_t)c1 | (uint32_t)c2 << 16;  // (at most kPass * kFinish each)
+      sh.counts[turn][wave][1] = (uint32_t)c3;
+    }
+    __syncthreads();  // (the other turn's counts have been read by all when this one's are complete)
+    const uint32_t a = all_lanes<16>(sh.counts[turn][lane & 15][0], add);
+    const int n1 = (int)(a & 0xffff), n2 = (int)(a >> 16), n3 = (int)all_lanes<16>(sh.counts[turn][lane & 15][1], add);
+    const int t = n3 >= k ? 3 : n2 >= k ? 2 : n1 >= k ? 1 : 0;
+    bound |= (uint32_t)t << bit;
+    if (t) have = t == 3 ? n3 : t == 2 ? n2 : n1;
+    bit -= 2;
+    turn ^= 1;
+  }
+#pragma unroll 1
+  for (int i = tid; i < n; i += kFinish)
+    if (value(i) >= bound) sh.found[atomicAdd(&sh.n, 1)] = i;
   __syncthreads();
-  return dm_wave_max<16>(red[threadIdx.x & 15]);
+  // every wavefront has all of them in its lanes and ranks its share
+  const int mine = lane < have ? sh.found[lane] : 0;
+  const uint32_t v = lane < have ? sh.key[mine] : 0;
+#pragma unroll 1
+  for (int e = wave; e < have; e += kFinish / 64) {
+    const int i = __builtin_amdgcn_readlane(mine, e);
+    const uint32_t iv = (uint32_t)__builtin_amdgcn_readlane((int)v, e);
+    const int rank = __popcll(__builtin_amdgcn_ballot_w64(lane < have && (v > iv || (v == iv && mine < i))));
+    if (lane == 0 && rank < k) {
+      sh.list[rank] = i;
+      if (rank == k - 1) sh.least = iv;
+    }
+  }
+  __syncthreads();
+  return sh.least;
 }
 
 // grid (rows)
 template <bool F32>
 __global__ __launch_bounds__(kFinish) void logprobs_finish_kernel(LogprobArgs p) {
   using R = Row<F32>;
-  constexpr int PER = R::PER;
-  __shared__ float red[16];
-  __shared__ uint32_t keys[kGroups];
-  __shared__ int chosen[kMaxTop];          // groups, ascending
-  __shared__ uint32_t cand_o[kCands];
-  __shared__ uint32_t cand_i[kCands];
-  __shared__ int n_cands, count[2], fill[17];
-  __shared__ uint32_t least;               // order of the k-th best group's best
+  constexpr int PER = R::PER, SHIFT = F32 ? 0 : 16;  // (a bf16's order is in its upper half)
+  __shared__ float4 red[kFinish / 64];
+  __shared__ Select sel;
+  __shared__ int groups[kMaxTop], n_cands;
+  __shared__ uint32_t cand_o[kCands], cand_i[kCands];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const size_t row = blockIdx.x;
   const R r(p, row);
 
-  if (p.k) {
-    for (int g = tid; g < p.groups; g += kFinish) keys[g] = p.best[row * p.groups + g];
-    if (tid < kMaxTop) chosen[tid] = 0x7fffffff;
-    if (tid == 0) n_cands = 0;
-  }
-  // the row's sums, and the tokens that were asked for
-  float m = -DM_INF, l = 0.f, s = 0.f, c = 0.f;
+  // everything that does not wait for something else is asked for first
   float4 part = make_float4(-DM_INF, 0.f, 0.f, 0.f);
-  if (tid < p.runs) part = p.sums[row * p.runs + tid];  // (runs <= kGroups <= the workgroup)
-  m = wg_max(part.x, red);
+  if (tid < p.runs) part = p.sums[row * p.runs + tid];  // (runs <= the workgroup)
+  if (p.k)
+#pragma unroll 1
+    for (int i = tid; i < p.groups; i += kFinish) sel.key[i] = p.best[row * p.groups + i] >> SHIFT;
+  float asked = -DM_INF;
+  if (tid < p.n_tokens) {
+    const uint32_t t = p.tokens[row * p.n_tokens + tid];
+    if (t < (uint32_t)p.V) asked = r.at(t);
+  }
+  if (tid == 0) n_cands = 0;
+  // the row's sums
+  const float wm = dm_wave_max<64>(part.x);
+  if (part.x < wm) move_to(wm, part.x, part.y, part.z, part.w);
+  part = make_float4(wm, dm_wave_sum<64>(part.y), dm_wave_sum<64>(part.z), dm_wave_sum<64>(part.w));
+  if (lane == 0) red[wave] = part;
+  __syncthreads();
+  part = red[lane & 15];
+  const float m = dm_wave_max<16>(part.x);
   if (part.x < m) move_to(m, part.x, part.y, part.z, part.w);
-  l = wg_sum(part.y, red);
-  s = wg_sum(part.z, red);
-  c = wg_sum(part.w, red);
+  const float s = dm_row_sum(part.z), l = dm_fma(kLn2, dm_fma(kL2ELow, s, dm_row_sum(part.w)), dm_row_sum(part.y));
   const float ref = m > -DM_INF ? m : 0.f;
-  l = dm_fma(kLn2, dm_fma(kL2ELow, s, c), l);
   const bool none = l == 0.f;
   const float logl = none ? 0.f : dm_log(l);
   if (tid == 0) {
@@ -220,138 +324,101 @@ __global__ __launch_bounds__(kFinish) void logprobs_finish_kernel(LogprobArgs p)
     if (p.entropy) p.entropy[row] = none ? 0.f : logl - s / l;
   }
   for (int i = tid; i < p.n_tokens; i += kFinish) {
-    const uint32_t t = p.tokens[row * p.n_tokens + i];
-    p.logprobs[row * p.n_tokens + i] = t < (uint32_t)p.V ? (r.at(t) - ref) - logl : -DM_INF;
+    if (i != tid) {
+      const uint32_t t = p.tokens[row * p.n_tokens + i];
+      asked = t < (uint32_t)p.V ? r.at(t) : -DM_INF;
+    }
+    p.logprobs[row * p.n_tokens + i] = (asked - ref) - logl;
   }
   if (p.k == 0) return;
 
-  // the k best groups: a group's rank is how many come before it, counted by 1024 / 512 threads each
-  const int kg = min(p.k, p.groups);
+  // the best groups
+  const int kg = min(p.k, p.groups), np = kg * kGroupPieces;
+  uint32_t least = select_best(p.groups, kg, sel);
+  if (tid < kg) groups[tid] = sel.list[tid];
+  if (kg < p.k) least = 0;  // (fewer groups than alternatives: all of their tokens)
+  __syncthreads();
+  auto piece_of = [&](int i) { return groups[i / kGroupPieces] * kGroupPieces + i % kGroupPieces; };
+  // their tokens that reach the bound of the groups: mostly not many more than k, and those are ranked
   {
-    const int g = tid >> 1, part_of = tid & 1;
-    int rank = 0;
-    const uint32_t mine = g < p.groups ? keys[g] : 0;
-    const int half = (p.groups + 1) / 2, lo = part_of * half, hi = min(p.groups, lo + half);
-    for (int o = lo; o < hi; ++o) rank += keys[o] > mine || (keys[o] == mine && o < g);
-    rank += __shfl_xor(rank, 1, 64);
-    __syncthreads();
-    if (g < p.groups && part_of == 0 && rank < kg) chosen[rank] = g;
-    if (g < p.groups && part_of == 0 && rank == kg - 1) least = mine;
-  }
-  __syncthreads();
-  // in ascending order, so that places in the list go with token ids
-  if (tid < 64) {
-    const int g = tid < kg ? chosen[tid] : 0x7fffffff;
-    int rank = 0;
-    for (int o = 0; o < kg; ++o) rank += __builtin_amdgcn_readlane(g, o) < g;
-    if (tid < kg) chosen[rank] = g;
-  }
-  __syncthreads();
-
-  // the tokens of those groups: who is at least as good as the k-th group's best
-  const int ppg = 64 * p.steps, pieces = kg * ppg;  // 16-byte pieces
-  auto piece_of = [&](int i) { return chosen[i / ppg] * ppg + i % ppg; };
-  const uint32_t bound = kg < p.k ? 0 : least;  // (fewer groups than alternatives: all of their tokens)
-  // the lanes that have one put it into the list, which has no order: it is ranked by value and id
-  auto push = [&](bool has, uint32_t o, int t) {
-    const uint64_t mask = __builtin_amdgcn_ballot_w64(has);
-    if (mask == 0) return;
-    int at = 0;
-    if (lane == 0) at = atomicAdd(&n_cands, __popcll(mask));
-    at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((uint64_t(1) << lane) - 1));
-    if (has && at < kCands) {
-      cand_o[at] = o;
-      cand_i[at] = t;
-    }
-  };
-  // every token of the chosen groups, in passes of 1024 pieces that all threads go through
-  auto look = [&](auto&& f) {
-    for (int i0 = 0; i0 < pieces; i0 += kFinish) {
-      const int i = i0 + tid;
-      float x[PER] = {};
-      int t0 = p.V;
-      if (i < pieces) {
-        const int piece = piece_of(i);
-        r.load(piece, x);
-        t0 = r.first(piece);
-      }
+    float next[PER];
+    const int i_first = wave * 64;
+    if (i_first < np) r.load(piece_of(i_first) + lane, next);
+#pragma unroll 1
+    for (int i0 = i_first; i0 < np; i0 += kFinish) {
+      const int t0 = r.first(piece_of(i0) + lane);
+      float x[PER];
 #pragma unroll
-      for (int e = 0; e < PER; ++e) f(t0 + e >= 0 && t0 + e < p.V, order_of(x[e]), t0 + e);
-    }
-  };
-  look([&](bool in, uint32_t o, int t) { push(in && o >= bound, o, t); });
-  __syncthreads();
-  int n = n_cands;
-  if (n > kCands) {
-    // Many equal tokens, or many good ones in one group: the k-th best value is found bit by bit, then
-    // all that are better are taken and, of its equals, those of the lowest ids.
-    uint32_t kth = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t tryit = kth | 1u << bit;
-      int have = 0;
-      look([&](bool in, uint32_t o, int) { have += in && o >= tryit; });
-      if (tid < 2) count[tid] = 0;
-      __syncthreads();
-      for (int sft = 32; sft; sft >>= 1) have += __shfl_xor(have, sft, 64);
-      if (lane == 0) atomicAdd(&count[0], have);
-      __syncthreads();
-      if (count[0] >= p.k) kth = tryit;
-      __syncthreads();
-    }
-    if (tid == 0) n_cands = 0;
-    if (tid == 0) count[1] = 0;
-    __syncthreads();
-    // the better ones (fewer than k) first: any order
-    look([&](bool in, uint32_t o, int t) { push(in && o > kth, o, t); });
-    __syncthreads();
-    const int better = n_cands;
-    // the equals in the order of their ids: passes of 1024 pieces, a prefix sum over the workgroup each
-    for (int i0 = 0; i0 < pieces; i0 += kFinish) {
-      const int i = i0 + tid;
-      uint32_t equal = 0;
-      int t0 = 0;
-      if (i < pieces) {
-        const int piece = piece_of(i);
-        float x[PER];
-        r.load(piece, x);
-        t0 = r.first(piece);
+      for (int e = 0; e < PER; ++e) x[e] = next[e];
+      if (i0 + kFinish < np) r.load(piece_of(i0 + kFinish) + lane, next);
 #pragma unroll
-        for (int e = 0; e < PER; ++e) equal |= (uint32_t)(order_of(x[e]) == kth && t0 + e >= 0 && t0 + e < p.V) << e;
-      }
-      const int mine = __popc(equal);
-      int before = mine;  // inclusive over the wavefront
-      for (int sft = 1; sft < 64; sft <<= 1) {
-        const int o = __shfl_up(before, sft, 64);
-        if (lane >= sft) before += o;
-      }
-      if (lane == 63) fill[wave] = before;
-      __syncthreads();
-      int at = better + count[1] + before - mine;
-      for (int wv = 0; wv < wave; ++wv) at += fill[wv];
-      for (int e = 0; e < PER; ++e)
-        if (equal >> e & 1) {
-          if (at < p.k) {
-            cand_o[at] = kth;
+      for (int e = 0; e < PER; ++e) {
+        const uint32_t o = order_of(x[e]);
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(r.has(t0 + e) && o >> SHIFT >= least);
+        if (mask) {
+          int at = 0;
+          if (lane == 0) at = atomicAdd(&n_cands, __popcll(mask));
+          at = __builtin_amdgcn_readfirstlane(at) + __popcll(mask & ((uint64_t(1) << lane) - 1));
+          if ((mask >> lane & 1) && at < kCands) {
+            cand_o[at] = o;
             cand_i[at] = t0 + e;
           }
-          ++at;
         }
-      __syncthreads();
-      if (tid == 0)
-        for (int wv = 0; wv < 16; ++wv) count[1] += fill[wv];
-      __syncthreads();
-      if (better + count[1] >= p.k) break;
+      }
     }
-    n = p.k;
   }
-  // rank them
-  for (int i = tid; i < n; i += kFinish) {
+  __syncthreads();
+  const bool by_piece = n_cands > kCands;
+  if (by_piece) {
+    // Equal tokens without end, or many good ones in one group: the best pieces first. The groups in
+    // ascending order, so that equal pieces are taken in the order of their tokens.
+    if (wave == 0) {
+      const int g = lane < kg ? sel.list[lane] : 0x7fffffff;
+      int place = 0;
+#pragma unroll 1
+      for (int o = 0; o < kg; ++o) place += __builtin_amdgcn_readlane(g, o) < g;
+      if (lane < kg) groups[place] = g;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < np; i += kFinish) {
+      const int piece = piece_of(i);
+      float x[PER];
+      r.load(piece, x);
+      uint32_t best = 0;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) best = max(best, r.has(r.first(piece) + e) ? order_of(x[e]) >> SHIFT : 0u);
+      sel.key[i] = best;
+    }
+    __syncthreads();
+    least = select_best(np, p.k, sel);
+  }
+  if (by_piece) {
+    // (the row has k tokens or more, but not always k pieces: then all of them)
+    if (tid == 0) n_cands = 0;
+    __syncthreads();
+    if (tid < p.k * PER) {
+      const int t = r.first(piece_of(sel.list[tid / PER])) + tid % PER;
+      const uint32_t o = r.has(t) ? order_of(r.at(t)) : 0;
+      if (r.has(t) && o >> SHIFT >= least) {
+        const int at = atomicAdd(&n_cands, 1);
+        cand_o[at] = o;
+        cand_i[at] = t;
+      }
+    }
+    __syncthreads();
+  }
+  const int n = n_cands;
+  for (int i = wave; i < n; i += kFinish / 64) {
     const uint32_t o = cand_o[i], id = cand_i[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += cand_o[j] > o || (cand_o[j] == o && cand_i[j] < id);
-    if (rank < p.k) {
+    for (int j0 = 0; j0 < n; j0 += 64) {
+      const int j = j0 + lane;
+      rank += __popcll(__builtin_amdgcn_ballot_w64(j < n && (cand_o[j] > o || (cand_o[j] == o && cand_i[j] < id))));
+    }
+    if (lane == 0 && rank < p.k) {
       p.top_ids[row * p.k + rank] = id;
-      p.top_logprobs[row * p.k + rank] = (r.at(id) - ref) - logl;
+      p.top_logprobs[row * p.k + rank] = (value_of(o) - ref) - logl;
     }
   }
 }
@@ -368,6 +435,7 @@ extern "C" int ornith_token_logprobs(ornith_ctx* ctx, const void* d_logits, int 
   ORN_REQUIRE(k >= 0 && k <= kMaxTop && k <= V, "token_logprobs: %d alternatives of %d tokens (at most %d)", k, V, kMaxTop);
   ORN_REQUIRE(k == 0 || (d_top_ids && d_top_logprobs), "token_logprobs: alternatives without their arrays");
   ORN_REQUIRE(((uintptr_t)d_logits & (dtype == ORNITH_F32 ? 3 : 1)) == 0, "token_logprobs: misaligned logits");
+  ORN_REQUIRE(V <= kMaxV, "token_logprobs: %d logits a row (at most %d)", V, kMaxV);
   ORN_REQUIRE(ctx, "token_logprobs: null context");
   const OrnDevice on(ctx);
   LogprobArgs p{};
@@ -382,14 +450,11 @@ extern "C" int ornith_token_logprobs(ornith_ctx* ctx, const void* d_logits, int 
   p.V = V;
   p.n_tokens = n_tokens;
   p.k = k;
-  // groups of 2 KB, longer ones only where a row would have more than kGroups of them
   const int per = dtype == ORNITH_F32 ? 4 : 8;
   const int64_t pieces = ((int64_t)V + 2 * per - 2) / per;  // at any alignment
-  p.steps = 2;
-  while ((pieces + 64 * p.steps - 1) / (64 * p.steps) > kGroups) p.steps *= 2;
-  p.groups = (int)((pieces + 64 * p.steps - 1) / (64 * p.steps));
+  p.groups = (int)((pieces + kGroupPieces - 1) / kGroupPieces);
   // a wavefront takes one group while that fills the machine, eight where there are rows enough
-  p.run = (int)std::min<int64_t>(8, std::max<int64_t>(1, (int64_t)rows * p.groups / (32 * ctx->compute_units)));
+  p.run = (int)std::min<int64_t>(8, std::max<int64_t>((p.groups + kFinish - 1) / kFinish, (int64_t)rows * p.groups / (32 * ctx->compute_units)));
   p.runs = (p.groups + p.run - 1) / p.run;
   void* base = nullptr;
   if (int rc = ornith_scratch(ctx, (size_t)rows * (p.runs * sizeof(float4) + p.groups * 4) + 512, &base)) return rc;
