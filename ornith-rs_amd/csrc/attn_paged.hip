@@ -117,15 +117,31 @@ struct PagedArgs {
   float c2;                 // scale * log2(e)
 };
 
-__device__ __forceinline__ void wg_barrier() {
+// What this wavefront (or, with a barrier, the workgroup) has read of LDS is in registers: it may be written again.
+template <bool SHARED_BLOCK>
+__device__ __forceinline__ void reads_done() {
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);
+  if (SHARED_BLOCK) __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
-// all but the last N of this wavefront's loads have arrived
+// The results of matrix instructions may be read eight wait states after the last of them (16 x 16 x 32). Where
+// the reader is in another block that two paths lead to, the compiler counts along one of them only and
+// leaves the shorter one without its wait: a row's maximum was then now and then taken from a partial
+// sum, which moved the reference point of its exponentials and with it the last bits of the result.
 template <int N>
+__device__ __forceinline__ void settle(f32x4_t (&v)[N]) {
+  static_assert(N == 1 || N == 4, "of a block's scores");
+  if constexpr (N == 1) asm volatile("s_nop 7" : "+v"(v[0]));
+  else asm volatile("s_nop 7" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+}
+// All but the last N of this wavefront's (the workgroup's wavefronts') loads have arrived.
+template <int N, bool SHARED_BLOCK>
 __device__ __forceinline__ void wait_loads() {
+  asm volatile("" ::: "memory");
   __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4 << 14) | 7 << 4 | 15 << 8);
+  if (SHARED_BLOCK) __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // What a row's result is made of by its last step: o / l, the gate, one rounding.
@@ -134,58 +150,62 @@ __device__ __forceinline__ float finish_value(float o, float inv, float gate, bo
   return gated ? y / (1.0f + __builtin_amdgcn_exp2f(-gate * 1.44269504088896341f)) : y;
 }
 
-// RW wavefronts of 16 query rows each share a block of BK keys; KW such sets take the chunk's blocks in
-// turn and meet at the end.
+// A workgroup of four wavefronts works in one of two forms:
+//   RW = 4, BK = 64  four wavefronts of 16 query rows share a block of 64 keys
+//   RW = 1, BK = 16  16 query rows; every wavefront has a block of 16 keys of its own in turn, and their
+//                    sums meet at the end (few rows: what counts is how much is in flight)
+// Both take 64 KB of LDS at a head width of 256, two workgroups a compute unit.
 //
 // Both products run transposed, so that a lane owns a query row from the scores to the output and the
 // probabilities never leave the registers:
 //   S^T[key, row] = K . Q^T    A = 16 keys x 32 channels from LDS, B = the row's channels (registers)
-//   O^T[ch, row] += V^T . P^T  A = 16 channels x 32 keys, B = the lane's eight probabilities
+//   O^T[ch, row] += V^T . P^T  A = 16 channels x 32 (16) keys, B = the lane's eight (four) probabilities
 // The lane of group g = lane / 16 holds keys 16 n + 4 g + r of its row's scores; an MFMA does not care
 // in which order k runs if both operands agree, so the k order of the second product is that of the
 // registers: keys 4 g .. + 4 and 16 + 4 g .. + 4 of 32. V^T's eight are two transposing LDS reads of
 // four keys each (ds_read_b64_tr_b16), so that K and V both lie in LDS as they do in memory and go there
 // without passing a register (buffer loads to LDS; rows past the end read as zeros).
 // 32-byte pieces of a row lie permuted by its number, so that eight rows' same piece is on all banks.
-template <int HD, int RW, int KW, int BK>
-struct Attend {
-  static constexpr int NT = 64 * RW * KW, ROWB = HD * 2, TILE = BK * ROWB, NS = HD / 32, NC = HD / 16, NK = BK / 16;
-  static constexpr int LPR = HD / 8;            // lanes a row in a load to LDS
-  static constexpr int LOADS = TILE / 1024 / RW;  // loads a wavefront makes for a block of keys (or values)
-  static constexpr int STAGE = 2 * TILE * KW;
-  static constexpr int JOIN = KW > 1 ? KW * RW * 16 * (HD * 4 + 8) : 0;
-  static constexpr int LDS = STAGE > JOIN ? STAGE : JOIN;
-  static_assert(TILE % (1024 * RW) == 0, "whole loads");
+constexpr int kWaves = 4;
 
-  // which 32-byte slot of its row piece c (of 16 bytes) of row `key` lies in, as a byte offset
-  static __device__ __forceinline__ int swz(int key) { return HD >= 128 ? key & 7 : key >> 1 & 3; }
+template <int HD, int RW, int BK>
+struct Attend {
+  static constexpr int KW = kWaves / RW, ROWB = HD * 2, TILE = BK * ROWB, NS = HD / 32, NC = HD / 16, NK = BK / 16;
+  static constexpr int LPR = HD / 8, RPL = 64 / LPR;  // lanes a row, rows a load to LDS
+  static constexpr int GROUPS = BK / 16 / RW;         // of 16 rows, which lie on one page, that a wavefront fetches of a block
+  static constexpr int PER_GROUP = 16 / RPL, LOADS = GROUPS * PER_GROUP;
+  static constexpr int STAGE = 2 * TILE * KW;
+  static constexpr int JOIN = KW > 1 ? kWaves * 16 * (HD * 4 + 8) : 0;
+  static constexpr int LDS = STAGE > JOIN ? STAGE : JOIN;
+  static_assert(BK % (16 * RW) == 0 && (BK == 16 || BK % 32 == 0), "whole groups");
+
+  // which 32-byte slot of a row its first one lies in
+  static __device__ __forceinline__ int swz(int row) { return HD >= 128 ? row & 7 : row >> 1 & 3; }
 };
 
-template <int HD, int RW, int KW, int BK, bool SHARED>
-__global__ __launch_bounds__(64 * RW * KW, KW == 1 ? 2 : 1) void attend_kernel(PagedArgs p) {
-  using A = Attend<HD, RW, KW, BK>;
-  constexpr int ROWB = A::ROWB, TILE = A::TILE, NS = A::NS, NC = A::NC, NK = A::NK;
-  extern __shared__ __align__(1024) unsigned char lds[];
-  __shared__ uint32_t ids[kChunkPages];
+template <int HD, int RW, int BK, bool SHARED>
+__device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsigned char* lds, uint32_t* ids) {
+  using A = Attend<HD, RW, BK>;
+  constexpr int ROWB = A::ROWB, TILE = A::TILE, NS = A::NS, NC = A::NC, NK = A::NK, KW = A::KW;
   const int G = p.Hq / p.l.Hkv, rows = (SHARED ? p.b.B : 1) * p.T * G, tiles = (rows + 16 * RW - 1) / (16 * RW);
   // the tiles of one chunk and KV head go to one die, next to each other: they read the same keys
-  const int die = blockIdx.x % kDies, nth = blockIdx.x / kDies, round = nth / tiles, tile = nth - round * tiles;
+  const int die = block % kDies, nth = block / kDies, round = nth / tiles, tile = nth - round * tiles;
   int item = round * kDies + die;
-  const int chunks = p.chunks[SHARED ? 0 : 1], seqs = SHARED ? 1 : p.b.B;
+  const int chunk_len = p.chunk[SHARED ? 0 : 1], chunks = p.chunks[SHARED ? 0 : 1], seqs = SHARED ? 1 : p.b.B;
   if (item >= chunks * seqs * p.l.Hkv) return;
   const int hk = item % p.l.Hkv;
   item /= p.l.Hkv;
   const int chunk = item / seqs, seq = item - chunk * seqs;
-  const int k0 = (SHARED ? 0 : p.shared) + chunk * p.chunk[SHARED ? 0 : 1];
-  const int k1 = min(k0 + p.chunk[SHARED ? 0 : 1], SHARED ? p.shared : batch_len(p.b, seq));
+  const int k0 = (SHARED ? 0 : p.shared) + chunk * chunk_len;
+  const int k1 = min(k0 + chunk_len, SHARED ? p.shared : batch_len(p.b, seq));
   const bool finishes = p.chunks[0] + p.chunks[1] == 1;
   if (k0 >= k1 && !finishes) return;  // (no key of the chunk: the join knows)
 
   const int lane = threadIdx.x & 63, l16 = lane & 15, lg = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = KW == 1 ? 0 : wave / RW, rw = wave - set * RW;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), set = KW == 1 ? 0 : wave, rw = KW == 1 ? wave : 0;
   // the chunk's page ids
   const int page0 = k0 >> p.l.shift, npages = ((k1 - 1) >> p.l.shift) - page0 + 1;
-  for (int i = threadIdx.x; i < npages; i += A::NT)
+  for (int i = threadIdx.x; i < npages; i += 64 * kWaves)
     ids[i] = min(p.b.table[(size_t)seq * p.b.stride + page0 + i], (uint32_t)p.l.n_pages - 1);
 
   // this lane's query row
@@ -200,50 +220,76 @@ __global__ __launch_bounds__(64 * RW * KW, KW == 1 ? 2 : 1) void attend_kernel(P
 
   unsigned char* const kt = lds + set * 2 * TILE;
   unsigned char* const vt = kt + TILE;
-  const size_t head_rows = (size_t)1 << p.l.shift;
-  // block `blk` of keys or values: piece i of 1 KB holds 1024 / ROWB rows
-  auto fetch = [&](const bf16_t* pool, unsigned char* to, int blk) {
-    constexpr int RPL = 1024 / ROWB;
+  // The byte of a group's memory that the lane takes in load i: row i RPL + lane / LPR, the piece that its slot
+  // in LDS holds. The numbers' bits lie apart, so load i's is load 0's with a constant's bits turned.
+  const int lr = lane / A::LPR, slot = lane % A::LPR;
+  const uint32_t at0 = lr * ROWB + 32 * ((slot >> 1) ^ A::swz(lr)) + 16 * (slot & 1);
+  // the page of 16-row group g of this wavefront's part of a block (any id where there is no key)
+  auto page_of = [&](int blk, int g) {
+    const int key = k0 + blk * BK + 16 * (g * RW + rw);
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)ids[min((key >> p.l.shift) - page0, kChunkPages - 1)]);
+  };
+  auto fetch = [&](const bf16_t* pool, unsigned char* to, int blk, const uint32_t (&page)[A::GROUPS]) {
 #pragma unroll
-    for (int i = 0; i < A::LOADS; ++i) {
-      const int row0 = (i * RW + rw) * RPL, key = k0 + blk * BK + row0;  // (k0 and blocks are multiples of the rows a load has)
-      const bool some = key < k1;
-      const uint32_t id = __builtin_amdgcn_readfirstlane(some ? ids[(key >> p.l.shift) - page0] : 0u);
-      const int in_page = key & ((1 << p.l.shift) - 1);
-      const bf16_t* base = pool + (((size_t)id * p.l.Hkv + hk) * head_rows + (some ? in_page : 0)) * HD;
-      const __amdgpu_buffer_rsrc_t buf = dm_buffer(base, some ? min(RPL, k1 - key) * ROWB : 0);
-      const int lr = lane / A::LPR, slot = lane % A::LPR;
-      const int c = ((slot >> 1) ^ A::swz(row0 + lr)) * 2 + (slot & 1);
-      typedef __attribute__((address_space(3))) void lds_t;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_t*)(to + (i * RW + rw) * 1024), 16, lr * ROWB + 16 * c, 0, 0, 0);
+    for (int g = 0; g < A::GROUPS; ++g) {
+      const int key = k0 + blk * BK + 16 * (g * RW + rw), have = min(16, k1 - key);
+      const size_t first = ((((size_t)page[g] * p.l.Hkv + hk) << p.l.shift) + (key & ((1 << p.l.shift) - 1))) * HD;
+      const __amdgpu_buffer_rsrc_t buf = dm_buffer(pool + (have > 0 ? first : 0), have > 0 ? have * ROWB : 0);
+#pragma unroll
+      for (int i = 0; i < A::PER_GROUP; ++i) {
+        typedef __attribute__((address_space(3))) void lds_t;
+        const uint32_t turned = (uint32_t)(i * A::RPL * ROWB + 32 * A::swz(i * A::RPL));
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_t*)(to + (g * RW + rw) * 16 * ROWB + i * 1024), 16, at0 ^ turned, 0, 0, 0);
+      }
     }
   };
+  static_assert(ROWB * A::RPL == 1024 && (HD < 128 || A::RPL <= 4), "a load is 1 KB of rows; its first row's number ends in zeros");
 
   f32x4_t o[NC];
 #pragma unroll
   for (int t = 0; t < NC; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m_i = -DM_INF, l_i = 0.f;
   const int blocks = (k1 - k0 + BK - 1) / BK, turns = (blocks + KW - 1) / KW;
-  fetch(p.l.k, kt, set);
-  fetch(p.l.v, vt, set);
+  uint32_t page[A::GROUPS];
+#pragma unroll
+  for (int g = 0; g < A::GROUPS; ++g) page[g] = page_of(set, g);
+  fetch(p.l.k, kt, set, page);
+  fetch(p.l.v, vt, set, page);
+#pragma unroll 1
   for (int turn = 0; turn < turns; ++turn) {
     const int blk = turn * KW + set, key0 = k0 + blk * BK;
-    wait_loads<A::LOADS>();
-    wg_barrier();
+#pragma unroll
+    for (int g = 0; g < A::GROUPS; ++g) page[g] = page_of(blk + KW, g);
+    wait_loads<A::LOADS, KW == 1>();
+    // ---- S^T = K Q^T, the fragments of a step leaving LDS under the products of the step before
     f32x4_t st[NK];
 #pragma unroll
     for (int n = 0; n < NK; ++n) st[n] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    {
+      constexpr int STEP = NS < 4 / NK ? NS : 4 / NK, FR = STEP * NK;  // channels' steps at a time: four fragments
+      bf16x8_t kf[2][FR];
+      auto read = [&](int s, bf16x8_t (&f)[FR]) {
 #pragma unroll
-    for (int ks = 0; ks < NS; ++ks)
+        for (int u = 0; u < FR; ++u) {
+          const int key = 16 * (u % NK) + l16, c = 4 * (s * STEP + u / NK) + lg;
+          f[u] = *reinterpret_cast<const bf16x8_t*>(kt + key * ROWB + (((c >> 1) ^ A::swz(key)) << 5) + ((c & 1) << 4));
+        }
+      };
+      static_assert(NS % STEP == 0 && 4 % NK == 0, "whole steps");
+      read(0, kf[0]);
 #pragma unroll
-      for (int n = 0; n < NK; ++n) {
-        const int key = 16 * n + l16, c = 4 * ks + lg;
-        const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kt + key * ROWB + (((c >> 1) ^ A::swz(key)) << 5) + ((c & 1) << 4));
-        st[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[ks], st[n], 0, 0, 0);
+      for (int s = 0; s < NS / STEP; ++s) {
+        if (s + 1 < NS / STEP) read(s + 1, kf[(s + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < FR; ++u)
+          st[u % NK] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[s & 1][u], qf[s * STEP + u / NK], st[u % NK], 0, 0, 0);
       }
-    wg_barrier();
-    fetch(p.l.k, kt, blk + KW);
-    // the online softmax of the lane's row: the reference point of its exponentials moves when the
+    }
+    settle(st);
+    reads_done<KW == 1>();
+    fetch(p.l.k, kt, blk + KW, page);
+    // ---- the online softmax of the lane's row: the reference point of its exponentials moves when the
     // maximum has grown by more than 8 binary orders (probabilities up to 2^8 do no harm, and the
     // final division takes them out)
     float mx = -DM_INF;
@@ -280,8 +326,7 @@ __global__ __launch_bounds__(64 * RW * KW, KW == 1 ? 2 : 1) void attend_kernel(P
 #pragma unroll
       for (int t = 0; t < NC; ++t) o[t] *= alpha;
     }
-    wait_loads<A::LOADS>();
-    wg_barrier();
+    wait_loads<A::LOADS, KW == 1>();
     // A key that one row of the tile sees and another does not: its probability is 0 there, but 0
     // times a value that is no finite number is none. Blocks with such keys (the last of a sequence)
     // are looked through. If there is one, the product leaves out what is not finite, and that is added
@@ -289,6 +334,7 @@ __global__ __launch_bounds__(64 * RW * KW, KW == 1 ? 2 : 1) void attend_kernel(P
     bool odd = false;
     if (masked && __builtin_amdgcn_ballot_w64(vis > 0 && vis < min(key0 + BK, k1)) != 0) {
       uint32_t bad = 0;
+#pragma unroll 1
       for (int i = lane; i < TILE / 16; i += 64) {
         const u32x4_t w = *reinterpret_cast<const u32x4_t*>(vt + 16 * i);
 #pragma unroll
@@ -296,35 +342,50 @@ __global__ __launch_bounds__(64 * RW * KW, KW == 1 ? 2 : 1) void attend_kernel(P
       }
       odd = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
     }
-    bf16x8_t pb[BK / 32];
-#pragma unroll
-    for (int k2 = 0; k2 < BK / 32; ++k2) {
-      u32x4_t w;
-      w[0] = dm_f2bf2(st[2 * k2][0], st[2 * k2][1]);
-      w[1] = dm_f2bf2(st[2 * k2][2], st[2 * k2][3]);
-      w[2] = dm_f2bf2(st[2 * k2 + 1][0], st[2 * k2 + 1][1]);
-      w[3] = dm_f2bf2(st[2 * k2 + 1][2], st[2 * k2 + 1][3]);
-      pb[k2] = __builtin_bit_cast(bf16x8_t, w);
-    }
+    // ---- O^T += V^T P^T
     auto product = [&](auto only_finite) {
+      constexpr bool FINITE = decltype(only_finite)::value;
+      constexpr int KG = BK == 16 ? 1 : 2;  // groups of four keys a lane has of a fragment
+      uint32_t pb[BK / 8];                  // pairs of probabilities
 #pragma unroll
-      for (int k2 = 0; k2 < BK / 32; ++k2)
+      for (int n = 0; n < NK; ++n) {
+        pb[2 * n] = dm_f2bf2(st[n][0], st[n][1]);
+        pb[2 * n + 1] = dm_f2bf2(st[n][2], st[n][3]);
+      }
+      s16x4_t vf[2][4][KG];
+      constexpr int BATCHES = NK / KG * NC / 4;  // of four fragments
+      auto read = [&](int b, s16x4_t (&f)[4][KG]) {
 #pragma unroll
-        for (int t = 0; t < NC; ++t) {
-          s16x4_t h[2];
+        for (int u = 0; u < 4; ++u)
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int key = 32 * k2 + 16 * u + 4 * lg + (l16 >> 2);
+          for (int h = 0; h < KG; ++h) {
+            const int t = (4 * b + u) % NC, kg = (4 * b + u) / NC, key = 16 * KG * kg + 16 * h + 4 * lg + (l16 >> 2);
             typedef __attribute__((address_space(3))) s16x4_t lds4;
-            h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vt + key * ROWB + ((t ^ A::swz(key)) << 5) + 8 * (l16 & 3)));
-            if constexpr (decltype(only_finite)::value) {
+            f[u][h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(vt + key * ROWB + ((t ^ A::swz(key)) << 5) + 8 * (l16 & 3)));
+            if constexpr (FINITE) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) h[u][e] = (h[u][e] & 0x7f80) == 0x7f80 ? (short)0 : h[u][e];
+              for (int e = 0; e < 4; ++e) f[u][h][e] = (f[u][h][e] & 0x7f80) == 0x7f80 ? (short)0 : f[u][h][e];
             }
           }
-          const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
-          o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[k2], o[t], 0, 0, 0);
+      };
+      read(0, vf[0]);
+#pragma unroll
+      for (int b = 0; b < BATCHES; ++b) {
+        if (b + 1 < BATCHES) read(b + 1, vf[(b + 1) & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int t = (4 * b + u) % NC, kg = (4 * b + u) / NC;
+          if constexpr (KG == 1) {
+            const s16x4_t pv = __builtin_bit_cast(s16x4_t, u32x2_t{pb[0], pb[1]});
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf[b & 1][u][0], pv, o[t], 0, 0, 0);
+          } else {
+            const bf16x8_t v = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(vf[b & 1][u][0], vf[b & 1][u][KG - 1], 0, 1, 2, 3, 4, 5, 6, 7));
+            const bf16x8_t pv = __builtin_bit_cast(bf16x8_t, u32x4_t{pb[4 * kg], pb[4 * kg + 1], pb[4 * kg + 2], pb[4 * kg + 3]});
+            o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pv, o[t], 0, 0, 0);
+          }
         }
+      }
     };
     if (!odd) {
       product(std::false_type{});
@@ -349,30 +410,30 @@ __global__ __launch_bounds__(64 * RW * KW, KW == 1 ? 2 : 1) void attend_kernel(P
         }
       }
     }
-    wg_barrier();
-    fetch(p.l.v, vt, blk + KW);
+    reads_done<KW == 1>();
+    fetch(p.l.v, vt, blk + KW, page);
   }
-  wait_loads<0>();  // (the last turns' requests write zeros: not into the LDS of whoever comes next)
+  wait_loads<0, false>();  // (the last turns' requests write zeros: not into the LDS of whoever comes next)
   l_i = l_i + dm_xor_lane<16>(l_i);
   l_i = l_i + dm_xor_lane<32>(l_i);
 
   int t_lo = 0;  // the first of the channel tiles that this wavefront goes on with
   if constexpr (KW > 1) {
-    // the sets' sums meet: every wavefront leaves its own in LDS and takes a share of the channels of all
-    static_assert(NC % KW == 0, "whole channel tiles a set");
-    wg_barrier();
+    // the wavefronts' sums meet: each leaves its own in LDS and takes a share of the channels of all
+    static_assert(NC % KW == 0, "whole channel tiles a wavefront");
+    __syncthreads();
     f32x4_t* const ob = reinterpret_cast<f32x4_t*>(lds);
-    float2* const ml = reinterpret_cast<float2*>(lds + (size_t)KW * RW * 16 * HD * 4);
+    float2* const ml = reinterpret_cast<float2*>(lds + (size_t)KW * 16 * HD * 4);
 #pragma unroll
-    for (int t = 0; t < NC; ++t) ob[((set * RW + rw) * NC + t) * 64 + lane] = o[t];
-    if (lg == 0) ml[(set * RW + rw) * 16 + l16] = make_float2(m_i, l_i);
+    for (int t = 0; t < NC; ++t) ob[(set * NC + t) * 64 + lane] = o[t];
+    if (lg == 0) ml[set * 16 + l16] = make_float2(m_i, l_i);
     __syncthreads();
     float w[KW], m = -DM_INF, l = 0.f;
 #pragma unroll
-    for (int s = 0; s < KW; ++s) m = fmaxf(m, ml[(s * RW + rw) * 16 + l16].x);
+    for (int s = 0; s < KW; ++s) m = fmaxf(m, ml[s * 16 + l16].x);
 #pragma unroll
     for (int s = 0; s < KW; ++s) {
-      const float2 v = ml[(s * RW + rw) * 16 + l16];
+      const float2 v = ml[s * 16 + l16];
       w[s] = v.x > -DM_INF ? __builtin_amdgcn_exp2f((v.x - m) * p.c2) : v.y != v.y ? 1.f : 0.f;
       l += v.y * w[s];
     }
@@ -384,7 +445,7 @@ __global__ __launch_bounds__(64 * RW * KW, KW == 1 ? 2 : 1) void attend_kernel(P
       f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < KW; ++s) {
-        const f32x4_t v = ob[((s * RW + rw) * NC + t_lo + u) * 64 + lane];
+        const f32x4_t v = ob[(s * NC + t_lo + u) * 64 + lane];
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] = dm_fma(v[e], w[s], sum[e]);
       }
@@ -392,11 +453,11 @@ __global__ __launch_bounds__(64 * RW * KW, KW == 1 ? 2 : 1) void attend_kernel(P
     }
   }
   if (rho >= rows) return;
-  const int nt = KW > 1 ? NC / KW : NC;
+  constexpr int NT = KW > 1 ? NC / KW : NC;
   if (finishes) {
     const float inv = vis > 0 && l_i != 0.f ? 1.0f / l_i : 0.f;
 #pragma unroll
-    for (int u = 0; u < nt; ++u) {
+    for (int u = 0; u < NT; ++u) {
       const int ch = 16 * (t_lo + u) + 4 * lg;
       u32x2_t gw = {0, 0};
       if (p.qg) gw = *reinterpret_cast<const u32x2_t*>(p.qg + row_head * 2 * HD + HD + ch);
@@ -410,31 +471,90 @@ __global__ __launch_bounds__(64 * RW * KW, KW == 1 ? 2 : 1) void attend_kernel(P
   }
   const size_t at = (size_t)((SHARED ? 0 : p.chunks[0]) + chunk) * p.b.B * p.T * p.Hq + row_head;
 #pragma unroll
-  for (int u = 0; u < nt; ++u) *reinterpret_cast<f32x4_t*>(p.part_o + at * HD + 16 * (t_lo + u) + 4 * lg) = o[u];
+  for (int u = 0; u < NT; ++u) *reinterpret_cast<f32x4_t*>(p.part_o + at * HD + 16 * (t_lo + u) + 4 * lg) = o[u];
   if (lg == 0 && t_lo == 0) p.part_ml[at] = make_float2(m_i, l_i);
 }
 
-// Joins the slots of a (row, head): four channels a lane. Chunks past what the row sees were not
-// computed for it, or hold nothing of it, and are not read.
 template <int HD>
-__global__ __launch_bounds__(HD / 4) void join_kernel(PagedArgs p) {
-  const int r = blockIdx.y, head = blockIdx.x, ch = 4 * threadIdx.x, seq = r / p.T;
+constexpr int attend_lds() {
+  constexpr int wide = Attend<HD, 4, 64>::LDS, narrow = Attend<HD, 1, 16>::LDS;
+  return wide > narrow ? wide : narrow;
+}
+
+// Workgroups below `split` have chunks of the shared part, the others of the sequences' own.
+template <int HD, bool WIDE_SHARED, bool WIDE_OWN>
+__global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(PagedArgs p, int split) {
+  __shared__ __align__(1024) unsigned char lds[attend_lds<HD>()];
+  __shared__ uint32_t ids[kChunkPages];
+  if ((int)blockIdx.x < split) attend_part<HD, WIDE_SHARED ? 4 : 1, WIDE_SHARED ? 64 : 16, true>(p, blockIdx.x, lds, ids);
+  else attend_part<HD, WIDE_OWN ? 4 : 1, WIDE_OWN ? 64 : 16, false>(p, blockIdx.x - split, lds, ids);
+}
+
+// Joins the slots of a (row, head): four channels a lane, the slots dealt to the wavefronts, whose sums
+// meet in LDS. Chunks past what the row sees were not computed for it, or hold nothing of it, and are
+// not read.
+constexpr int kJoinWaves = 4;
+template <int HD>
+__global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedArgs p) {
+  constexpr int LANES = HD / 4, PARTS = 64 * kJoinWaves / LANES;
+  __shared__ float4 so[PARTS][LANES];
+  __shared__ float2 sml[PARTS];
+  const int r = blockIdx.y, head = blockIdx.x, part = threadIdx.x / LANES, ch = 4 * (threadIdx.x % LANES), seq = r / p.T;
   const int vis = batch_len(p.b, seq) - p.T + (r - seq * p.T) + 1;
   const size_t row_head = (size_t)r * p.Hq + head, slot = (size_t)p.b.B * p.T * p.Hq;
   const int ns = vis > 0 ? min(p.chunks[0], (vis + p.chunk[0] - 1) / p.chunk[0]) : 0;
   const int no = vis > p.shared ? min(p.chunks[1], (vis - p.shared + p.chunk[1] - 1) / p.chunk[1]) : 0;
   auto place = [&](int i) { return (size_t)(i < ns ? i : p.chunks[0] + i - ns) * slot + row_head; };
+  // the slots of this part, four at a time: a running maximum as over keys
   float m = -DM_INF, l = 0.f;
-  for (int i = 0; i < ns + no; ++i) m = fmaxf(m, p.part_ml[place(i)].x);
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < ns + no; ++i) {
-    const float2 v = p.part_ml[place(i)];
-    const float w = v.x > -DM_INF ? __builtin_amdgcn_exp2f((v.x - m) * p.c2) : v.y != v.y ? 1.f : 0.f;
-    l = dm_fma(v.y, w, l);
-    if (w != 0.f) {
-      const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p.part_o + place(i) * HD + ch);
+  for (int i0 = part; i0 < ns + no; i0 += 4 * PARTS) {
+    float2 v[4];
+    f32x4_t x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = dm_fma(x[e], w, o[e]);
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * PARTS;
+      v[u] = make_float2(-DM_INF, 0.f);
+      x[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (i < ns + no) {
+        v[u] = p.part_ml[place(i)];
+        x[u] = *reinterpret_cast<const f32x4_t*>(p.part_o + place(i) * HD + ch);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (i0 + u * PARTS >= ns + no) continue;
+      const float mn = fmaxf(m, v[u].x);
+      const float a = m > -DM_INF ? __builtin_amdgcn_exp2f((m - mn) * p.c2) : 1.f;  // (nothing yet, or NaN, which stays)
+      const float w = v[u].x > -DM_INF ? __builtin_amdgcn_exp2f((v[u].x - mn) * p.c2) : v[u].y != v[u].y ? 1.f : 0.f;
+      m = mn;
+      l = dm_fma(v[u].y, w, l * a);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = w != 0.f ? dm_fma(x[u][e], w, o[e] * a) : o[e] * a;
+    }
+  }
+  if constexpr (PARTS > 1) {
+    so[part][ch / 4] = make_float4(o[0], o[1], o[2], o[3]);
+    if (ch == 0) sml[part] = make_float2(m, l);
+    __syncthreads();
+    if (part) return;
+    float mt = -DM_INF;
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) mt = fmaxf(mt, sml[q].x);
+    l = 0.f;
+    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+      const float2 v = sml[q];
+      const float4 x = so[q][ch / 4];
+      const float w = v.x > -DM_INF ? __builtin_amdgcn_exp2f((v.x - mt) * p.c2) : v.y != v.y ? 1.f : 0.f;
+      l = dm_fma(v.y, w, l);
+      if (w != 0.f) {
+        o[0] = dm_fma(x.x, w, o[0]);
+        o[1] = dm_fma(x.y, w, o[1]);
+        o[2] = dm_fma(x.z, w, o[2]);
+        o[3] = dm_fma(x.w, w, o[3]);
+      }
     }
   }
   const float inv = l != 0.f ? 1.0f / l : 0.f;
@@ -446,39 +566,27 @@ __global__ __launch_bounds__(HD / 4) void join_kernel(PagedArgs p) {
   *reinterpret_cast<u32x2_t*>(p.out + row_head * HD + ch) = u32x2_t{dm_f2bf2(y[0], y[1]), dm_f2bf2(y[2], y[3])};
 }
 
-template <int HD, int RW, int KW, int BK, bool SHARED>
-int launch_part(ornith_ctx* ctx, const PagedArgs& a) {
-  using A = Attend<HD, RW, KW, BK>;
-  const void* f = reinterpret_cast<const void*>(attend_kernel<HD, RW, KW, BK, SHARED>);
-  if (A::LDS > 65536 - 4 * kChunkPages) ORN_HIP(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, A::LDS));
-  const int64_t rows = (int64_t)(SHARED ? a.b.B : 1) * a.T * (a.Hq / a.l.Hkv), tiles = (rows + 16 * RW - 1) / (16 * RW);
-  const int64_t items = (int64_t)a.chunks[SHARED ? 0 : 1] * (SHARED ? 1 : a.b.B) * a.l.Hkv;
-  hipLaunchKernelGGL((attend_kernel<HD, RW, KW, BK, SHARED>), dim3((unsigned)((items + kDies - 1) / kDies * kDies * tiles)), dim3(A::NT), A::LDS,
-                     ctx->stream, a);
-  ORN_LAUNCH_CHECK("attend_kernel");
-  return ORNITH_OK;
-}
-
 template <int HD>
 int attend(ornith_ctx* ctx, PagedArgs a, int max_rows) {
-  const int G = a.Hq / a.l.Hkv, own_rows = a.T * G, shared_rows = a.b.B * own_rows;
-  // chunks: enough workgroups for every compute unit, no chunk shorter than 256 keys
-  auto cut = [&](int part, int keys, int64_t sharers, int rows_a_wg) {
-    if (keys <= 0) {
-      a.chunk[part] = 1;
-      a.chunks[part] = 0;
-      return;
-    }
-    const int64_t wgs = sharers * rows_a_wg;
-    const int want = (int)std::max<int64_t>(1, (2 * ctx->compute_units + wgs - 1) / wgs);
-    // (whole blocks of 64; a chunk that begins inside a page touches one page more than it has)
-    const int most = ((kChunkPages - 1) << a.l.shift) / 64 * 64, len = std::min(std::max(256, ((keys + want - 1) / want + 63) / 64 * 64), most);
+  const int own_rows = a.T * (a.Hq / a.l.Hkv), shared_rows = a.b.B * own_rows;
+  const bool wide[2] = {shared_rows > 32, own_rows > 32};
+  int64_t grid[2];
+  const int keys[2] = {a.shared, max_rows - a.shared}, rows[2] = {shared_rows, own_rows}, seqs[2] = {1, a.b.B};
+  for (int part = 0; part < 2; ++part) {
+    // chunks: two workgroups for every compute unit, no chunk shorter than 128 keys; whole blocks of 64 (a
+    // chunk that begins inside a page touches one page more than it has)
+    const int tile = wide[part] ? 64 : 16, most = ((kChunkPages - 1) << a.l.shift) / 64 * 64;
+    const int64_t tiles = (rows[part] + tile - 1) / tile, pairs = (int64_t)seqs[part] * a.l.Hkv;
+    const int64_t want = std::max<int64_t>(1, (2 * ctx->compute_units + tiles * pairs - 1) / (tiles * pairs));
+    const int len = (int)std::min<int64_t>(std::max<int64_t>(128, ((keys[part] + want - 1) / want + 63) / 64 * 64), most);
     a.chunk[part] = len;
-    a.chunks[part] = (keys + len - 1) / len;
-  };
-  const bool wide_shared = shared_rows > 32, wide_own = own_rows > 32;
-  cut(0, a.shared, a.l.Hkv, wide_shared ? (shared_rows + 63) / 64 : (shared_rows + 15) / 16);
-  cut(1, max_rows - a.shared, (int64_t)a.l.Hkv * a.b.B, wide_own ? (own_rows + 63) / 64 : (own_rows + 15) / 16);
+    a.chunks[part] = (keys[part] + len - 1) / len;
+    grid[part] = (a.chunks[part] * pairs + kDies - 1) / kDies * kDies * tiles;
+  }
+  if (a.chunks[0] + a.chunks[1] == 0) {  // max_rows is 0: no row sees anything
+    a.chunks[1] = 1;
+    grid[1] = ((int64_t)a.b.B * a.l.Hkv + kDies - 1) / kDies * kDies * ((own_rows + (wide[1] ? 63 : 15)) / (wide[1] ? 64 : 16));
+  }
   const int slots = a.chunks[0] + a.chunks[1];
   const size_t cells = (size_t)a.b.B * a.T * a.Hq;
   if (slots != 1) {
@@ -488,12 +596,13 @@ int attend(ornith_ctx* ctx, PagedArgs a, int max_rows) {
     a.part_o = sc.take<float>(slots * cells * HD);
     a.part_ml = sc.take<float2>(slots * cells);
   }
-  if (a.chunks[0])
-    if (int rc = wide_shared ? launch_part<HD, 4, 1, 64, true>(ctx, a) : launch_part<HD, 1, 4, 32, true>(ctx, a)) return rc;
-  if (a.chunks[1])
-    if (int rc = wide_own ? launch_part<HD, 4, 1, 64, false>(ctx, a) : launch_part<HD, 1, 4, 32, false>(ctx, a)) return rc;
+  void (*const kernel)(PagedArgs, int) = wide[0] ? wide[1] ? attend_kernel<HD, true, true> : attend_kernel<HD, true, false>
+                                                 : wide[1] ? attend_kernel<HD, false, true> : attend_kernel<HD, false, false>;
+  ORN_REQUIRE(grid[0] + grid[1] <= INT32_MAX, "sdpa_paged: %lld workgroups", (long long)(grid[0] + grid[1]));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(grid[0] + grid[1])), dim3(64 * kWaves), 0, ctx->stream, a, (int)grid[0]);
+  ORN_LAUNCH_CHECK("attend_kernel");
   if (slots != 1) {
-    hipLaunchKernelGGL(join_kernel<HD>, dim3(a.Hq, a.b.B * a.T), dim3(HD / 4), 0, ctx->stream, a);
+    hipLaunchKernelGGL(join_kernel<HD>, dim3(a.Hq, a.b.B * a.T), dim3(64 * kJoinWaves), 0, ctx->stream, a);
     ORN_LAUNCH_CHECK("join_kernel");
   }
   return ORNITH_OK;
