@@ -144,10 +144,22 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("" ::: "memory");
 }
 
-// What a row's result is made of by its last step: o / l, the gate, one rounding.
-__device__ __forceinline__ float finish_value(float o, float inv, float gate, bool gated) {
-  const float y = o * inv;
-  return gated ? y / (1.0f + __builtin_amdgcn_exp2f(-gate * 1.44269504088896341f)) : y;
+// The last step of four channels of a row: values / sum (a row that sees nothing has no sum: zeros), the gate, one rounding.
+template <int HD>
+__device__ __forceinline__ void store_result(const PagedArgs& p, size_t row_head, int ch, const f32x4_t& o, float l) {
+  const float inv = l != 0.f ? 1.0f / l : 0.f;
+  float y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = l != 0.f ? o[e] * inv : 0.f;
+  if (p.qg) {
+    const u32x2_t gw = *reinterpret_cast<const u32x2_t*>(p.qg + row_head * 2 * HD + HD + ch);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float g = e & 1 ? dm_bf2f_hi(gw[e >> 1]) : dm_bf2f_lo(gw[e >> 1]);
+      y[e] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-g * 1.44269504088896341f));
+    }
+  }
+  *reinterpret_cast<u32x2_t*>(p.out + row_head * HD + ch) = u32x2_t{dm_f2bf2(y[0], y[1]), dm_f2bf2(y[2], y[3])};
 }
 
 // A workgroup of four wavefronts works in one of two forms:
@@ -218,8 +230,6 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
   for (int ks = 0; ks < NS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8_t*>(p.q + row_head * HD + 32 * ks + 8 * lg);
   __syncthreads();
 
-  unsigned char* const kt = lds + set * 2 * TILE;
-  unsigned char* const vt = kt + TILE;
   // The byte of a group's memory that the lane takes in load i: row i RPL + lane / LPR, the piece that its slot
   // in LDS holds. The numbers' bits lie apart, so load i's is load 0's with a constant's bits turned.
   const int lr = lane / A::LPR, slot = lane % A::LPR;
@@ -253,6 +263,9 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
   uint32_t page[A::GROUPS];
 #pragma unroll
   for (int g = 0; g < A::GROUPS; ++g) page[g] = page_of(set, g);
+  // (The two tiles come as parameters that are told apart: behind a request into LDS the compiler has every
+  // read of LDS that may be of the same bytes wait for all requests in flight.)
+  auto walk = [&](unsigned char* __restrict__ kt, unsigned char* __restrict__ vt) __attribute__((always_inline)) {
   fetch(p.l.k, kt, set, page);
   fetch(p.l.v, vt, set, page);
 #pragma unroll 1
@@ -390,7 +403,6 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
     if (!odd) {
       product(std::false_type{});
     } else {
-      product(std::true_type{});
 #pragma unroll 1
       for (int j = 0; j < BK; ++j) {
         float w = 0.f;
@@ -409,10 +421,13 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
           }
         }
       }
+      product(std::true_type{});
     }
     reads_done<KW == 1>();
     fetch(p.l.v, vt, blk + KW, page);
   }
+  };
+  walk(lds + set * 2 * TILE, lds + set * 2 * TILE + TILE);
   wait_loads<0, false>();  // (the last turns' requests write zeros: not into the LDS of whoever comes next)
   l_i = l_i + dm_xor_lane<16>(l_i);
   l_i = l_i + dm_xor_lane<32>(l_i);
@@ -455,18 +470,8 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
   if (rho >= rows) return;
   constexpr int NT = KW > 1 ? NC / KW : NC;
   if (finishes) {
-    const float inv = vis > 0 && l_i != 0.f ? 1.0f / l_i : 0.f;
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int ch = 16 * (t_lo + u) + 4 * lg;
-      u32x2_t gw = {0, 0};
-      if (p.qg) gw = *reinterpret_cast<const u32x2_t*>(p.qg + row_head * 2 * HD + HD + ch);
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        y[e] = vis > 0 ? finish_value(o[u][e], inv, e & 1 ? dm_bf2f_hi(gw[e >> 1]) : dm_bf2f_lo(gw[e >> 1]), p.qg != nullptr) : 0.f;
-      *reinterpret_cast<u32x2_t*>(p.out + row_head * HD + ch) = u32x2_t{dm_f2bf2(y[0], y[1]), dm_f2bf2(y[2], y[3])};
-    }
+    for (int u = 0; u < NT; ++u) store_result<HD>(p, row_head, 16 * (t_lo + u) + 4 * lg, o[u], vis > 0 ? l_i : 0.f);
     return;
   }
   const size_t at = (size_t)((SHARED ? 0 : p.chunks[0]) + chunk) * p.b.B * p.T * p.Hq + row_head;
@@ -557,13 +562,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedArgs p) {
       }
     }
   }
-  const float inv = l != 0.f ? 1.0f / l : 0.f;
-  u32x2_t gw = {0, 0};
-  if (p.qg) gw = *reinterpret_cast<const u32x2_t*>(p.qg + row_head * 2 * HD + HD + ch);
-  float y[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = finish_value(o[e], inv, e & 1 ? dm_bf2f_hi(gw[e >> 1]) : dm_bf2f_lo(gw[e >> 1]), p.qg != nullptr);
-  *reinterpret_cast<u32x2_t*>(p.out + row_head * HD + ch) = u32x2_t{dm_f2bf2(y[0], y[1]), dm_f2bf2(y[2], y[3])};
+  store_result<HD>(p, row_head, ch, o, l);
 }
 
 template <int HD>
