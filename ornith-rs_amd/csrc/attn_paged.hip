@@ -144,6 +144,14 @@ __device__ __forceinline__ void wait_loads() {
   asm volatile("" ::: "memory");
 }
 
+// The least value among a wavefront's rows, one in each of N neighbouring lanes, the same in all groups of N.
+template <int N>
+__device__ __forceinline__ int least_of_rows(int v) {
+#pragma unroll
+  for (int s = N / 2; s; s >>= 1) v = min(v, __shfl_xor(v, s, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
 // The last step of four channels of a row: values / sum (a row that sees nothing has no sum: zeros), the gate, one rounding.
 template <int HD>
 __device__ __forceinline__ void store_result(const PagedArgs& p, size_t row_head, int ch, const f32x4_t& o, float l) {
@@ -224,6 +232,7 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
   const int rho = tile * 16 * RW + 16 * rw + l16, rc = (SHARED ? 0 : seq * p.T * G) + min(rho, rows - 1);
   const int r = rc / G, head = hk * G + (rc - r * G), rseq = r / p.T;
   const int vis = batch_len(p.b, rseq) - p.T + (r - rseq * p.T) + 1;  // keys that it sees
+  const int least_vis = least_of_rows<16>(vis);
   const size_t row_head = (size_t)r * p.Hq + head;
   bf16x8_t qf[NS];
 #pragma unroll
@@ -260,6 +269,8 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
   for (int t = 0; t < NC; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m_i = -DM_INF, l_i = 0.f;
   const int blocks = (k1 - k0 + BK - 1) / BK, turns = (blocks + KW - 1) / KW;
+  // turns whose blocks every row of the wavefronts sees in full: no masks, and no values to look through
+  const int whole = max(0, min(least_vis, k1) - k0) / (BK * KW);
   uint32_t page[A::GROUPS];
 #pragma unroll
   for (int g = 0; g < A::GROUPS; ++g) page[g] = page_of(set, g);
@@ -268,8 +279,8 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
   auto walk = [&](unsigned char* __restrict__ kt, unsigned char* __restrict__ vt) __attribute__((always_inline)) {
   fetch(p.l.k, kt, set, page);
   fetch(p.l.v, vt, set, page);
-#pragma unroll 1
-  for (int turn = 0; turn < turns; ++turn) {
+  auto one_block = [&](int turn, auto edge) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge)::value;
     const int blk = turn * KW + set, key0 = k0 + blk * BK;
 #pragma unroll
     for (int g = 0; g < A::GROUPS; ++g) page[g] = page_of(blk + KW, g);
@@ -307,7 +318,8 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
     // final division takes them out)
     float mx = -DM_INF;
     const int lim = min(vis, k1);  // (the shared part may end inside a block)
-    const bool masked = __builtin_amdgcn_ballot_w64(key0 + BK > lim) != 0;
+    bool masked = false;
+    if constexpr (EDGE) masked = __builtin_amdgcn_ballot_w64(key0 + BK > lim) != 0;
     if (masked) {
 #pragma unroll
       for (int n = 0; n < NK; ++n)
@@ -345,7 +357,7 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
     // are looked through. If there is one, the product leaves out what is not finite, and that is added
     // key by key to the rows that see it; the other rows keep their bits.
     bool odd = false;
-    if (masked && __builtin_amdgcn_ballot_w64(vis > 0 && vis < min(key0 + BK, k1)) != 0) {
+    if (EDGE && masked && __builtin_amdgcn_ballot_w64(vis > 0 && vis < min(key0 + BK, k1)) != 0) {
       uint32_t bad = 0;
 #pragma unroll 1
       for (int i = lane; i < TILE / 16; i += 64) {
@@ -400,7 +412,9 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
         }
       }
     };
-    if (!odd) {
+    if constexpr (!EDGE) {
+      product(std::false_type{});
+    } else if (!odd) {
       product(std::false_type{});
     } else {
 #pragma unroll 1
@@ -425,7 +439,12 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
     }
     reads_done<KW == 1>();
     fetch(p.l.v, vt, blk + KW, page);
-  }
+  };
+  int turn = 0;
+#pragma unroll 1
+  for (; turn < whole; ++turn) one_block(turn, std::false_type{});
+#pragma unroll 1
+  for (; turn < turns; ++turn) one_block(turn, std::true_type{});
   };
   walk(lds + set * 2 * TILE, lds + set * 2 * TILE + TILE);
   wait_loads<0, false>();  // (the last turns' requests write zeros: not into the LDS of whoever comes next)
