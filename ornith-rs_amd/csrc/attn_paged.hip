@@ -529,14 +529,14 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedArgs p) {
   const int ns = vis > 0 ? min(p.chunks[0], (vis + p.chunk[0] - 1) / p.chunk[0]) : 0;
   const int no = vis > p.shared ? min(p.chunks[1], (vis - p.shared + p.chunk[1] - 1) / p.chunk[1]) : 0;
   auto place = [&](int i) { return (size_t)(i < ns ? i : p.chunks[0] + i - ns) * slot + row_head; };
-  // the slots of this part, four at a time: a running maximum as over keys
+  // the slots of this part, eight at a time (few turns: each waits for memory): a running maximum as over keys
   float m = -DM_INF, l = 0.f;
   f32x4_t o = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = part; i0 < ns + no; i0 += 4 * PARTS) {
-    float2 v[4];
-    f32x4_t x[4];
+  for (int i0 = part; i0 < ns + no; i0 += 8 * PARTS) {
+    float2 v[8];
+    f32x4_t x[8];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < 8; ++u) {
       const int i = i0 + u * PARTS;
       v[u] = make_float2(-DM_INF, 0.f);
       x[u] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -546,7 +546,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedArgs p) {
       }
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < 8; ++u) {
       if (i0 + u * PARTS >= ns + no) continue;
       const float mn = fmaxf(m, v[u].x);
       const float a = m > -DM_INF ? __builtin_amdgcn_exp2f((m - mn) * p.c2) : 1.f;  // (nothing yet, or NaN, which stays)
@@ -591,12 +591,15 @@ int attend(ornith_ctx* ctx, PagedArgs a, int max_rows) {
   int64_t grid[2];
   const int keys[2] = {a.shared, max_rows - a.shared}, rows[2] = {shared_rows, own_rows}, seqs[2] = {1, a.b.B};
   for (int part = 0; part < 2; ++part) {
-    // chunks: two workgroups for every compute unit, no chunk shorter than 128 keys; whole blocks of 64 (a
-    // chunk that begins inside a page touches one page more than it has)
+    // chunks: two workgroups for every compute unit; whole blocks of 64 (a chunk that begins inside a page
+    // touches one page more than it has). None is shorter than 128 keys, 192 in the narrow form: with more of
+    // them the sums that go through memory cost more than the keys' reads gain (both launches, us, at least
+    // 64 / 128 / 192 / 256 keys: wide, 8 rows at 6600 keys, 20.8 / 16.7 / 17.7 / 17.4; narrow, 8 rows of 8 KV
+    // heads of 128 at 2300 keys, 13.8 / 12.3 / 10.8 / 10.9, 4 rows at 1000 keys, - / 10.5 / 10.6 / 11.3).
     const int tile = wide[part] ? 64 : 16, most = ((kChunkPages - 1) << a.l.shift) / 64 * 64;
     const int64_t tiles = (rows[part] + tile - 1) / tile, pairs = (int64_t)seqs[part] * a.l.Hkv;
     const int64_t want = std::max<int64_t>(1, (2 * ctx->compute_units + tiles * pairs - 1) / (tiles * pairs));
-    const int len = (int)std::min<int64_t>(std::max<int64_t>(128, ((keys[part] + want - 1) / want + 63) / 64 * 64), most);
+    const int len = (int)std::min<int64_t>(std::max<int64_t>(wide[part] ? 128 : 192, ((keys[part] + want - 1) / want + 63) / 64 * 64), most);
     a.chunk[part] = len;
     a.chunks[part] = (keys[part] + len - 1) / len;
     grid[part] = (a.chunks[part] * pairs + kDies - 1) / kDies * kDies * tiles;
