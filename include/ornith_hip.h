@@ -444,7 +444,7 @@ typedef struct ornith_kv_batch {
   const int32_t* d_lens;   /* [B] rows held, those of the call itself included */
   int shared_rows;         /* the first shared_rows rows (whole pages) are the same pages for all B:
                               they are read once for all, through the first sequence's table */
-  int max_rows;            /* no sequence holds more */
+  int max_rows;            /* no sequence holds more; at most 2^30 */
 } ornith_kv_batch;
 
 /* Page dst[i] := page src[i], the first `rows` rows of every head, in all layers; host id lists,
@@ -475,7 +475,9 @@ ORNITH_API int ornith_attn_prep_paged(ornith_ctx* ctx, const ornith_kv_pages* pa
  * [0, d_lens[b] - T + t]; a row that sees none gives zeros. out bf16 [B, T, Hq, hd] =
  * sigmoid(gate) * attention, gate in the second half of d_qg [B, T, Hq, 2*hd]; with d_qg null the
  * attention alone. scale > 0. Scores, softmax and sums are fp32, probabilities go to the matrix
- * cores as bf16: the results agree with ornith_sdpa_decode_gated's to rounding, not bit for bit. */
+ * cores as bf16: the results agree with ornith_sdpa_decode_gated's to rounding, not bit for bit.
+ * The sums of parts of the cache meet in the context's own memory: a call that needs more of it than
+ * any before waits for the stream while it is allocated anew. */
 ORNITH_API int ornith_sdpa_paged_gated(ornith_ctx* ctx, const ornith_kv_pages* pages, int layer, const ornith_kv_batch* batch,
                                        const void* d_q_rot, const void* d_qg, int T, int Hq, float scale, void* d_out);
 
@@ -546,9 +548,10 @@ ORNITH_API int ornith_argmax_rows(ornith_ctx* ctx, const void* d_logits, int row
  *   d_top_ids, d_top_logprobs [rows, k]  the k <= 32 most probable tokens, falling; equal logits by
  *                                the lower id; k may be 0 (both may be null)
  * A logit of -inf (a masked token) has probability 0 and log probability -inf; so has a token id
- * past the end. At most 65535 rows of 2097148 logits a call. A row of nothing but -inf has lse -inf and entropy 0. A row with a NaN or +inf
- * logit has no distribution: its lse, entropy and the log probabilities of its finite tokens are
- * not numbers (or -inf); the alternatives' ids still go by value, NaN last. */
+ * past the end. At most 65535 rows of 2097148 logits a call. A row of nothing but -inf has lse -inf
+ * and entropy 0. A row with a NaN or +inf logit has no distribution: its lse, entropy and the log
+ * probabilities of its finite tokens are not numbers (or -inf); the alternatives' ids still go by
+ * value, NaN last. Works in the context's own memory, as ornith_sdpa_paged_gated. */
 ORNITH_API int ornith_token_logprobs(ornith_ctx* ctx, const void* d_logits, int dtype, int rows, int V, int64_t row_stride,
                                      const uint32_t* d_tokens, int n_tokens, int k, float* d_logprobs, float* d_entropy, float* d_lse,
                                      uint32_t* d_top_ids, float* d_top_logprobs);

@@ -3,6 +3,7 @@
 // (KvCache::update_and_fetch, /root/reference/src/model/cache.rs:38-79; the reference has no pages).
 #include "kv_pages.h"
 
+#include <algorithm>
 #include <new>
 #include <vector>
 
@@ -76,7 +77,7 @@ int move_rows(ornith_ctx* ctx, const ornith_kv_pages* pages, int layer, const vo
   ORN_REQUIRE(rows >= 0 && row0 >= 0 && cap >= 0 && row0 <= cap - rows, "%s: rows [%d, +%d) of a cache of %d", who, row0, rows, cap);
   ORN_REQUIRE(n_ids >= 0 && (n_ids == 0 || ids), "%s: %d page ids without their array", who, n_ids);
   const int shift = kv_shift(pages->page_rows);
-  ORN_REQUIRE(at >= 0 && (int64_t)at + rows <= (int64_t)n_ids << shift, "%s: rows [%d, +%d) of %d pages of %d", who, at, rows, n_ids,
+  ORN_REQUIRE(at >= 0 && (int64_t)at + rows <= std::min<int64_t>((int64_t)n_ids << shift, 1 << 30), "%s: rows [%d, +%d) of %d pages of %d", who, at, rows, n_ids,
               pages->page_rows);
   if (rows == 0) return ORNITH_OK;
   ORN_REQUIRE(d_k && d_v && (((uintptr_t)d_k | (uintptr_t)d_v) & 15) == 0, "%s: null or misaligned cache", who);
@@ -133,6 +134,7 @@ int kv_batch_check(const ornith_kv_pages* p, const ornith_kv_batch* b, const cha
   ORN_REQUIRE(b, "%s: null batch", who);
   ORN_REQUIRE(b->B >= 1 && b->B <= 4096, "%s: %d sequences (1 to 4096)", who, b->B);
   ORN_REQUIRE(b->d_table && b->d_lens && b->table_stride >= 1, "%s: no page tables or lengths", who);
+  ORN_REQUIRE(b->max_rows <= 1 << 30, "%s: %d rows a sequence (at most 2^30)", who, b->max_rows);
   ORN_REQUIRE(b->max_rows >= 0 && b->max_rows <= (int64_t)b->table_stride * p->page_rows, "%s: %d rows in %d pages of %d", who, b->max_rows,
               b->table_stride, p->page_rows);
   ORN_REQUIRE(b->shared_rows >= 0 && b->shared_rows % p->page_rows == 0 && b->shared_rows <= b->max_rows,

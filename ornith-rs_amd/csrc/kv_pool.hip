@@ -47,6 +47,7 @@ struct ornith_kv_pool {
   std::vector<void*> k, v;
   std::vector<int> refs;  // sequences that hold a page; 0: free
   int n_free = 0;
+  uint32_t lowest = 0;    // no page below it is free
   std::vector<Seq> seqs;
   uint32_t* d_table = nullptr;  // [max_seqs, max_pages]
   uint32_t* d_batch = nullptr;  // [max_seqs, max_pages]
@@ -55,7 +56,10 @@ struct ornith_kv_pool {
   ornith_kv_pages pages() const { return ornith_kv_pages{n_layers, n_pages, page_rows, Hkv, hd, k.data(), v.data()}; }
   bool has(int s) const { return s >= 0 && s < max_seqs && seqs[s].open; }
   void drop(uint32_t page) {
-    if (--refs[page] == 0) ++n_free;
+    if (--refs[page] == 0) {
+      ++n_free;
+      lowest = std::min(lowest, page);
+    }
   }
 };
 
@@ -115,7 +119,7 @@ int ornith_kv_pool_create(ornith_ctx* ctx, int n_layers, int n_pages, int page_r
   ORN_REQUIRE(n_layers >= 1 && n_layers <= 4096, "kv_pool_create: %d layers", n_layers);
   ORN_REQUIRE(max_seqs >= 1 && max_seqs <= 4096 && max_pages >= 1 && max_pages <= n_pages, "kv_pool_create: %d sequences of %d pages (of %d)",
               max_seqs, max_pages, n_pages);
-  ORN_REQUIRE((int64_t)max_pages * page_rows <= INT32_MAX && (int64_t)max_seqs * max_pages <= INT32_MAX,
+  ORN_REQUIRE((int64_t)max_pages * page_rows <= 1 << 30 && (int64_t)max_seqs * max_pages <= INT32_MAX,
               "kv_pool_create: %d pages of %d rows for %d sequences", max_pages, page_rows, max_seqs);
   POOL_TRY("kv_pool_create", {
     // (the sizes' own checks, with pointers that stand for what is yet to be allocated)
@@ -222,8 +226,18 @@ int ornith_kv_pool_extend(ornith_kv_pool* p, const int* seqs, int n, int rows) {
     // what is needed: new pages, and copies of shared pages whose free rows will be written (the last
     // holder of one keeps it)
     std::vector<uint32_t> src, dst;
-    std::vector<int> left(p->refs);  // holders once the copies are made
     std::vector<char> copies(n);
+    // (a page's holders are counted down as their copies are planned, and up again if the call fails)
+    struct Planned {
+      ornith_kv_pool* p;
+      std::vector<uint32_t>& src;
+      bool done = false;
+      ~Planned() {
+        if (!done)
+          for (uint32_t id : src) ++p->refs[id];
+      }
+    } planned{p, src};
+    src.reserve(n);
     size_t need = 0;
     int most = 0;
     for (int i = 0; i < n; ++i) {
@@ -231,8 +245,8 @@ int ornith_kv_pool_extend(ornith_kv_pool* p, const int* seqs, int n, int rows) {
       const int64_t have = (int64_t)s.pages.size(), want = ((int64_t)s.rows + rows + p->page_rows - 1) / p->page_rows;
       ORN_REQUIRE(want <= p->max_pages, "kv_pool_extend: sequence %d would hold %lld pages of at most %d", seqs[i], (long long)want, p->max_pages);
       need += (size_t)(want - have);
-      if (s.rows % p->page_rows && left[s.pages.back()] > 1) {
-        --left[s.pages.back()];
+      if (s.rows % p->page_rows && p->refs[s.pages.back()] > 1) {
+        --p->refs[s.pages.back()];
         copies[i] = 1;
         src.push_back(s.pages.back());
         most = std::max(most, s.rows % p->page_rows);
@@ -242,19 +256,20 @@ int ornith_kv_pool_extend(ornith_kv_pool* p, const int* seqs, int n, int rows) {
     ORN_REQUIRE(need <= (size_t)p->n_free, "kv_pool_extend: %zu pages needed, %d of %d free", need, p->n_free, p->n_pages);
     for (int i = 0; i < n; ++i) p->seqs[seqs[i]].pages.reserve(((size_t)p->seqs[seqs[i]].rows + rows + p->page_rows - 1) / p->page_rows);
     std::vector<uint32_t> taken;
-    for (uint32_t id = 0; taken.size() < need; ++id)
+    for (uint32_t id = p->lowest; taken.size() < need; ++id)
       if (!p->refs[id]) taken.push_back(id);
     dst.assign(taken.begin(), taken.begin() + src.size());
     const ornith_kv_pages pages = p->pages();
     if (!src.empty())
       if (int rc = ornith_kv_pages_copy(p->ctx, &pages, src.data(), dst.data(), (int)src.size(), most)) return rc;
     // nothing below fails
+    planned.done = true;
     p->n_free -= (int)need;
+    if (need) p->lowest = taken.back() + 1;
     size_t c = 0, t = src.size();
     for (int i = 0; i < n; ++i) {
       Seq& s = p->seqs[seqs[i]];
       if (copies[i]) {
-        --p->refs[s.pages.back()];
         s.pages.back() = taken[c++];
         p->refs[s.pages.back()] = 1;
         s.synced = std::min(s.synced, s.pages.size() - 1);
@@ -310,6 +325,7 @@ int ornith_kv_pool_compact(ornith_kv_pool* p, int* moved) {
       to[src[i]] = dst[i];
       std::swap(p->refs[dst[i]], p->refs[src[i]]);
     }
+    p->lowest = used;
     for (Seq& s : p->seqs)
       for (size_t j = 0; j < s.pages.size(); ++j)
         if (s.pages[j] >= used) {

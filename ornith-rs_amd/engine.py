@@ -642,7 +642,7 @@ class KvPool:
     def close(self):
         if self.h:
             lib().ornith_kv_pool_destroy(self.h)
-            self.h = None
+            self.h, self.pages.s = None, KvPagesStruct()  # (calls over the pages that are gone are refused)
 
     def open(self):
         s = C.c_int()

@@ -398,3 +398,65 @@ def test_continuations_of_one_prompt(orn, ctx):
     assert pool.stats()[0] == 4                           # 207 rows of the one that was kept
     for d in (dk, dv, cos, sin, qw, kw): d.free()
     pool.close()
+
+
+def test_two_contexts(orn, ctx):
+    """Calls of two contexts, issued in turn and in flight together, each with partial sums of its own."""
+    other, rng = orn.Ctx(0), np.random.default_rng(29)
+    got = []
+    for x in (ctx, other):
+        cases = []
+        rng = np.random.default_rng(29)
+        for lens, T, shared in (([3000, 2500], 2, 2432), ([900] * 12, 4, 832), ([5000], 1, 0)):
+            c = Case(x, rng, lens, T, shared, 64, 16, 2, 256).upload(orn)
+            q = _bits(rng, (c.B, T, 16, 256))
+            cases.append((c, q, x.to_device(q), x.alloc(q.nbytes)))
+        got.append(cases)
+    for i in range(3):
+        for cases in got:
+            c, q, dq, out = cases[i]
+            c.ctx.sdpa_paged_gated(c.pages, 0, c.batch, dq, None, c.T, 16, 0.0625, out)
+    for i in range(3):
+        a, b = (cases[i][3].download(np.uint16, cases[i][1].shape) for cases in got)
+        c, q = got[0][i][:2]
+        want, tol = _want(c, q, None, 0.0625)
+        assert np.array_equal(a, b) and (np.abs(_f(a) - want) <= tol).all(), i
+    for cases in got:
+        for c, _, dq, out in cases: c.free(dq, out)
+    other.close()
+
+
+def test_pages_past_four_gigabytes(orn, ctx):
+    """Page ids whose bytes lie behind 2^32, in every call over pages: the same bits as at low ids."""
+    rng = np.random.default_rng(31)
+    lens, T, R, Hq, Hkv, hd, rope, big = [300, 257], 2, 64, 16, 2, 256, 64, 70000
+    low = Case(ctx, rng, lens, T, 128, R, Hq, Hkv, hd).upload(orn)
+    up = big - low.n_pages
+    k, v = (ctx.alloc(big * Hkv * R * hd * 2) for _ in range(2))
+    pages = orn.KvPages([k], [v], big, R, Hkv, hd)
+    one = [ctx.alloc(Hkv * R * hd * 2) for _ in range(2)]
+    named = sorted({int(i) for b in range(2) for i in low.table[b, :-(-lens[b] // R)]})
+    for i in named:
+        for x, a in zip(one, (low.k, low.v)): x.upload(a[0, i])
+        ctx.kv_pages_load(pages, 0, *one, R, 0, R, [i + up], 0)
+    table = low.table.copy()
+    table[table < low.n_pages] += np.uint32(up)
+    dt = ctx.to_device(table)
+    batch = orn.KvBatch(2, dt, low.stride, low.dl, 128, low.max_rows)
+    new = [ctx.to_device(_bits(rng, s)) for s in ((2, T, Hq, 2 * hd), (2, T, Hkv, hd), (2, T, Hkv, hd), (hd,), (hd,))]
+    cos, sin = ctx.rope_table(low.max_rows, rope, 1e4)
+    res = []
+    for p, b in ((low.pages, low.batch), (pages, batch)):
+        q, out = ctx.alloc(2 * T * Hq * hd * 2), ctx.alloc(2 * T * Hq * hd * 2)
+        ctx.attn_prep_paged(p, 0, b, *new, T, Hq, rope, 1e-6, cos, sin, low.max_rows, q)
+        ctx.sdpa_paged_gated(p, 0, b, q, new[0], T, Hq, 0.0625, out)
+        res.append([x.download(np.uint16, (2, T, Hq, hd)) for x in (q, out)])
+        for x in (q, out): x.free()
+    assert all(np.array_equal(a, b) for a, b in zip(*res)) and np.isfinite(_f(res[0][1])).all()
+    ctx.kv_pages_copy(pages, [i + up for i in named], [i + 7 for i in range(len(named))], R)
+    kv = [x.download(np.uint16, low.k.shape[1:]) for x in (low.dk[0], low.dv[0])]
+    for n, i in enumerate(named):
+        for page in (i + up, n + 7):
+            ctx.kv_pages_store(pages, 0, *one, R, 0, R, [page], 0)
+            for x, a in zip(one, kv): assert np.array_equal(x.download(np.uint16, (Hkv, R, hd)), a[i]), (i, page)
+    low.free(k, v, dt, cos, sin, *one, *new)

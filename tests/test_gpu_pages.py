@@ -191,3 +191,35 @@ def test_pool_refusals(orn, ctx):
     assert pool.stats() == (0, 0, 0)
     cache.free()
     pool.close()
+
+
+def test_pool_takes_the_lowest_pages(orn, ctx):
+    pool = orn.KvPool(ctx, 1, 40, 16, 1, 64, 6, 12)
+    a, b = pool.open(), pool.open()
+    pool.extend([a, b], 16 * 5)
+    assert list(pool.seq(a)[1]) == list(range(5)) and list(pool.seq(b)[1]) == list(range(5, 10))
+    pool.truncate(a, 16 * 2)                             # 2, 3, 4 are free
+    with pytest.raises(orn.OrnithError, match="at most 12"): pool.extend([a, b], 16 * 10)
+    pool.extend([b], 16 * 4)
+    assert list(pool.seq(b)[1]) == [5, 6, 7, 8, 9, 2, 3, 4, 10]
+    c, d = pool.fork(a, 2)
+    pool.extend([c, d], 17)
+    assert [list(pool.seq(s)[1]) for s in (c, d)] == [[0, 1, 11, 12], [0, 1, 13, 14]]
+    e, f = pool.fork(c, 2)                               # 12 holds one row and has three holders
+    with pytest.raises(orn.OrnithError, match="30 pages needed, 25 of 40 free"): pool.extend([c, e, f, d], 16 * 8 - 15)   # 7 each, 2 copies
+    assert pool.stats() == (15, 4, 6)
+    pool.extend([c, e, f], 1)                            # two of the three copy it
+    assert [int(pool.seq(s)[1][3]) for s in (c, e, f)] == [15, 16, 12] and pool.stats() == (17, 3, 6)
+    pool.close_seq(b)
+    assert pool.compact() == 6 and pool.stats()[0] == 8
+    pool.extend([a], 1)
+    assert list(pool.seq(a)[1]) == [0, 1, 8]
+    pool.close()
+
+
+def test_pages_of_a_closed_pool(orn, ctx):
+    pool = orn.KvPool(ctx, 1, 4, 16, 1, 64, 2, 4)
+    pages = pool.pages
+    pool.close()
+    with pytest.raises(orn.OrnithError, match="0 layers"): ctx.kv_pages_copy(pages, [0], [1], 16)
+    with pytest.raises(orn.OrnithError, match="no sequence 0"): pool.seq(0)

@@ -131,3 +131,15 @@ def test_pool_create(orn, args, text):
     h = C.c_void_p()
     _refused(orn, orn.lib().ornith_kv_pool_create(None, *args, C.byref(h)), text)
     assert not h.value
+
+
+def test_positions_past_thirty_bits(orn):
+    """Positions stay small enough for what is added to them."""
+    for call in (_sdpa, _prep):
+        _refused(orn, call(orn, _pages(orn), _batch(orn, stride=1 << 25, most=(1 << 30) + 1)), "at most 2^30")
+    ids = np.zeros((1 << 22) + 1, np.uint32)
+    for name in ("load", "store"):
+        _refused(orn, getattr(orn.lib(), "ornith_kv_pages_" + name)(None, C.byref(_pages(orn, page_rows=256).s), 0, C.c_void_p(0x1000), C.c_void_p(0x1000), 100, 0, 10,
+                                                                    ids.ctypes.data_as(C.c_void_p), ids.size, (1 << 30) - 9), "rows [1073741815, +10)")
+    h = C.c_void_p()
+    _refused(orn, orn.lib().ornith_kv_pool_create(None, 1, (1 << 22) + 1, 256, 1, 64, 1, (1 << 22) + 1, C.byref(h)), "4194305 pages of 256 rows")
