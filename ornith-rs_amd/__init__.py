@@ -413,27 +413,29 @@ class KvBatch:
 
 
 def _ids(a):
-    return np.ascontiguousarray(a, dtype=np.uint32)
+    """A list of page ids as (number, C array); the array keeps its own copy alive."""
+    a = np.array(a, dtype=np.uint32, order="C").reshape(-1)
+    return a.size, (C.c_uint32 * a.size).from_buffer(a) if a.size else None
 
 
 @_ctx_method
 def kv_pages_copy(self, pages, src, dst, rows):
-    src, dst = _ids(src), _ids(dst)
-    assert src.size == dst.size, (src.size, dst.size)
-    _check(lib().ornith_kv_pages_copy(self.h, C.byref(pages.s), _ptr(src), _ptr(dst), src.size, rows), "kv_pages_copy")
+    (n, src), (n_dst, dst) = _ids(src), _ids(dst)
+    assert n == n_dst, (n, n_dst)
+    _check(lib().ornith_kv_pages_copy(self.h, C.byref(pages.s), src, dst, n, rows), "kv_pages_copy")
 
 
 @_ctx_method
 def kv_pages_load(self, pages, layer, k_cache, v_cache, cap, row0, rows, ids, at):
-    ids = _ids(ids)
-    _check(lib().ornith_kv_pages_load(self.h, C.byref(pages.s), layer, k_cache.ptr, v_cache.ptr, cap, row0, rows, _ptr(ids), ids.size, at),
+    n, ids = _ids(ids)
+    _check(lib().ornith_kv_pages_load(self.h, C.byref(pages.s), layer, k_cache.ptr, v_cache.ptr, cap, row0, rows, ids, n, at),
            "kv_pages_load")
 
 
 @_ctx_method
 def kv_pages_store(self, pages, layer, k_cache, v_cache, cap, row0, rows, ids, at):
-    ids = _ids(ids)
-    _check(lib().ornith_kv_pages_store(self.h, C.byref(pages.s), layer, k_cache.ptr, v_cache.ptr, cap, row0, rows, _ptr(ids), ids.size, at),
+    n, ids = _ids(ids)
+    _check(lib().ornith_kv_pages_store(self.h, C.byref(pages.s), layer, k_cache.ptr, v_cache.ptr, cap, row0, rows, ids, n, at),
            "kv_pages_store")
 
 

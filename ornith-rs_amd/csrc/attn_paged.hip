@@ -38,10 +38,14 @@ struct AppendArgs {
   float eps;
 };
 
-// One wavefront a (head, row). The norm and the rotation stay fp32 and are rounded once, on the
-// store. (ornith_attn_prep rounds the norm's two products to bf16 as the reference's rms_norm does;
-// nothing here is compared bit for bit with a contiguous cache's rows, so the values keep what
-// they have.)
+// One wavefront a (head, row): inv = rsqrt(mean x^2 + eps), x inv w, and channel e turned against e + half by
+// the position's angle. A chain of latencies (length, page, row; norm across the lanes), with no work to
+// speak of: 3.2 us at 8 rows of 20 heads of 256 (160 KB), 4.5 us at 256 rows (5.2 MB; a copy of it takes
+// 1.1 us), where one launch after another takes 3.9 us either way. The row itself and the norm's weights
+// do not wait for the page: that took 0.6 us off.
+// The norm and the rotation stay fp32 and are rounded once, on the store. (ornith_attn_prep rounds the
+// norm's two products to bf16 as the reference's rms_norm does; nothing here is compared bit for bit with
+// a contiguous cache's rows, so the values keep what they have.)
 template <int PER>
 __global__ __launch_bounds__(64) void append_kernel(AppendArgs p) {
   constexpr int HD = 64 * PER;
@@ -50,6 +54,13 @@ __global__ __launch_bounds__(64) void append_kernel(AppendArgs p) {
   const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.l.Hkv;
   const int hk = is_q ? 0 : is_v ? h - p.Hq - p.l.Hkv : h - p.Hq;
   const bf16_t* src = is_q ? p.qg + ((size_t)row * p.Hq + h) * 2 * HD : (is_v ? p.vx : p.kx) + ((size_t)row * p.l.Hkv + hk) * HD;
+  float x[PER], w[PER];  // (asked for before the page is looked up)
+#pragma unroll
+  for (int i = 0; i < PER; ++i) x[i] = dm_bf2f(src[lane * PER + i]);
+  if (!is_v) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) w[i] = dm_bf2f((is_q ? p.qw : p.kw)[lane * PER + i]);
+  }
   bf16_t* dst;
   bool keep = pos >= 0 && (is_v || pos < p.npos);
   if (is_q) {
@@ -60,17 +71,13 @@ __global__ __launch_bounds__(64) void append_kernel(AppendArgs p) {
     dst = (is_v ? p.l.v : p.l.k) + ((((size_t)page * p.l.Hkv + hk) << p.l.shift) + (pos & ((1 << p.l.shift) - 1))) * HD;
   }
   if (!keep) return;
-  float x[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) x[i] = dm_bf2f(src[lane * PER + i]);
   if (!is_v) {
-    const bf16_t* w = is_q ? p.qw : p.kw;
     float a = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) a = dm_fma(x[i], x[i], a);
     const float inv = dm_rsqrt(dm_wave_sum<64>(a) / (float)HD + p.eps);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) x[i] = x[i] * inv * dm_bf2f(w[lane * PER + i]);
+    for (int i = 0; i < PER; ++i) x[i] = x[i] * inv * w[i];
     // channel e < half turns with e + half: `half` is a whole number of lanes
     const int hl = p.half / PER;
     const bool low = lane < hl, rot = lane < 2 * hl;
@@ -608,6 +615,7 @@ int attend(ornith_ctx* ctx, PagedArgs a, int max_rows) {
     a.chunks[1] = 1;
     grid[1] = ((int64_t)a.b.B * a.l.Hkv + kDies - 1) / kDies * kDies * ((own_rows + (wide[1] ? 63 : 15)) / (wide[1] ? 64 : 16));
   }
+  ORN_REQUIRE(grid[0] + grid[1] < int64_t(1) << 24, "sdpa_paged: %lld workgroups", (long long)(grid[0] + grid[1]));  // (2^32 threads a launch)
   const int slots = a.chunks[0] + a.chunks[1];
   const size_t cells = (size_t)a.b.B * a.T * a.Hq;
   if (slots != 1) {
@@ -619,7 +627,6 @@ int attend(ornith_ctx* ctx, PagedArgs a, int max_rows) {
   }
   void (*const kernel)(PagedArgs, int) = wide[0] ? wide[1] ? attend_kernel<HD, true, true> : attend_kernel<HD, true, false>
                                                  : wide[1] ? attend_kernel<HD, false, true> : attend_kernel<HD, false, false>;
-  ORN_REQUIRE(grid[0] + grid[1] <= INT32_MAX, "sdpa_paged: %lld workgroups", (long long)(grid[0] + grid[1]));
   hipLaunchKernelGGL(kernel, dim3((unsigned)(grid[0] + grid[1])), dim3(64 * kWaves), 0, ctx->stream, a, (int)grid[0]);
   ORN_LAUNCH_CHECK("attend_kernel");
   if (slots != 1) {
