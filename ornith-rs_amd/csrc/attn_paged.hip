@@ -594,15 +594,21 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedArgs p) {
 template <int HD>
 int attend(ornith_ctx* ctx, PagedArgs a, int max_rows) {
   const int own_rows = a.T * (a.Hq / a.l.Hkv), shared_rows = a.b.B * own_rows;
-  const bool wide[2] = {shared_rows > 32, own_rows > 32};
+  // Wide from more than 128 rows: below, the tiles of 16 rows read their keys out of the die's cache often
+  // enough, and their chunks are longer, so that less goes through memory. Both launches, us, narrow / wide,
+  // 2 KV heads of 256: 64 rows at 2000 keys 11.3 / 13.3, at 6621 17.1 / 16.8; 128 rows at 2000 12.9 / 14.8, at
+  // 6621 19.8 / 21.4, at 16300 26.8 / 32.1; 192 rows at 6621 23.4 / 25.3, at 16300 36.4 / 33.8; 256 rows at 6621
+  // 26.4 / 27.8, at 16300 34.9 / 34.4; 512 rows at 16300 54.8 / 43.
+  const bool wide[2] = {shared_rows > 128, own_rows > 128};
   int64_t grid[2];
   const int keys[2] = {a.shared, max_rows - a.shared}, rows[2] = {shared_rows, own_rows}, seqs[2] = {1, a.b.B};
   for (int part = 0; part < 2; ++part) {
-    // chunks: two workgroups for every compute unit; whole blocks of 64 (a chunk that begins inside a page
-    // touches one page more than it has). None is shorter than 128 keys, 192 in the narrow form: with more of
-    // them the sums that go through memory cost more than the keys' reads gain (both launches, us, at least
-    // 64 / 128 / 192 / 256 keys: wide, 8 rows at 6600 keys, 20.8 / 16.7 / 17.7 / 17.4; narrow, 8 rows of 8 KV
-    // heads of 128 at 2300 keys, 13.8 / 12.3 / 10.8 / 10.9, 4 rows at 1000 keys, - / 10.5 / 10.6 / 11.3).
+    // chunks: two workgroups for every compute unit (both launches, us, one / one and a half / two / three a
+    // unit: 512 rows at 16300 keys 44.3 / 41.7 / 43.5 / 48.6, 2048 at 32768 268 / 236 / 186 / 217); whole blocks of
+    // 64 (a chunk that begins inside a page touches one page more than it has). None is shorter than 128 keys,
+    // 192 in the narrow form: with more of them the sums that go through memory cost more than the keys'
+    // reads gain (at least 64 / 128 / 192 / 256 keys: wide, 64 rows at 6600 keys, 20.8 / 16.7 / 17.7 / 17.4; narrow, 32
+    // rows of 8 KV heads of 128 at 2300 keys, 13.8 / 12.3 / 10.8 / 10.9, 32 of 2 of 256 at 1000 keys, - / 10.5 / 10.6 / 11.3).
     const int tile = wide[part] ? 64 : 16, most = ((kChunkPages - 1) << a.l.shift) / 64 * 64;
     const int64_t tiles = (rows[part] + tile - 1) / tile, pairs = (int64_t)seqs[part] * a.l.Hkv;
     const int64_t want = std::max<int64_t>(1, (2 * ctx->compute_units + tiles * pairs - 1) / (tiles * pairs));
@@ -625,8 +631,9 @@ int attend(ornith_ctx* ctx, PagedArgs a, int max_rows) {
     a.part_o = sc.take<float>(slots * cells * HD);
     a.part_ml = sc.take<float2>(slots * cells);
   }
-  void (*const kernel)(PagedArgs, int) = wide[0] ? wide[1] ? attend_kernel<HD, true, true> : attend_kernel<HD, true, false>
-                                                 : wide[1] ? attend_kernel<HD, false, true> : attend_kernel<HD, false, false>;
+  // (the shared part has all sequences' rows: it is wide where a sequence's own part is)
+  void (*const kernel)(PagedArgs, int) =
+      wide[1] ? attend_kernel<HD, true, true> : wide[0] ? attend_kernel<HD, true, false> : attend_kernel<HD, false, false>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)(grid[0] + grid[1])), dim3(64 * kWaves), 0, ctx->stream, a, (int)grid[0]);
   ORN_LAUNCH_CHECK("attend_kernel");
   if (slots != 1) {

@@ -460,3 +460,23 @@ def test_pages_past_four_gigabytes(orn, ctx):
             ctx.kv_pages_store(pages, 0, *one, R, 0, R, [page], 0)
             for x, a in zip(one, kv): assert np.array_equal(x.download(np.uint16, (Hkv, R, hd)), a[i]), (i, page)
     low.free(k, v, dt, cos, sin, *one, *new)
+
+
+# more than 128 query rows a KV head: tiles of 64 rows, in the shared part alone or in the sequences' own too
+MANY = [(16, 2, 256), (24, 2, 128), (8, 1, 64)]
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", MANY)
+@pytest.mark.parametrize("lens,T,shared,R", [([300, 280, 10], 20, 256, 64), ([400 + 7 * i for i in range(20)], 1, 384, 64), ([90] * 9 + [0, 3, 128], 3, 64, 16), ([65], 33, 0, 16),
+                                             ([1100, 1025], 24, 1024, 256), ([130, 128, 129], 20, 128, 128)])
+def test_many_rows(orn, ctx, Hq, Hkv, hd, lens, T, shared, R):
+    rng = np.random.default_rng(hd + T)
+    c = Case(ctx, rng, lens, T, shared, R, Hq, Hkv, hd).upload(orn)
+    _check(orn, ctx, rng, c, std=2.0)
+    c.free()
+
+
+@pytest.mark.parametrize("Hq,Hkv,hd", MANY)
+@pytest.mark.parametrize("lens,T,shared", [([520, 700], 20, 512), ([300, 290], 25, 0), ([260] * 30, 2, 256)])
+def test_values_of_later_rows_stay_out_of_many(orn, ctx, Hq, Hkv, hd, lens, T, shared):
+    test_values_of_later_rows_stay_out(orn, ctx, Hq, Hkv, hd, lens, T, shared)
