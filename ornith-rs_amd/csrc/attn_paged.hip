@@ -512,6 +512,15 @@ constexpr int attend_lds() {
   return wide > narrow ? wide : narrow;
 }
 
+// What it measured, 16 query heads on 2 KV heads of 256, shared keys / own keys a sequence, both forms in one launch:
+//   2048 rows (64 sequences of 4 tokens x 8 heads), 32768 / 512   168-219 us by the card's clock, 640-830 TFLOP/s
+//   512 rows (16 x 4 x 8), 16256 / 77                             34 us, 500 TFLOP/s
+//   64 rows (8 x 1 x 8), 6592 / 200                               13-14 us, where a copy of its 16 MB takes 3.3
+// Wide: the matrix cores are busy a third of the time, LDS a third (V's transposing reads run at half the
+// rate of K's), half of the wavefronts' cycles are waits at the two barriers a block. With the fetches
+// taken out 185 us became 140, with V's reads 152, the softmax was within the noise. Larger tiles (128 rows, each
+// fragment of K and V for two products) were 188-195 us with twice the partial sums, 32 x 32 products slower.
+// Narrow: a chain of trips to memory, table, keys, values a turn; a workgroup has as much in flight as LDS holds.
 // Workgroups below `split` have chunks of the shared part, the others of the sequences' own.
 template <int HD, bool WIDE_SHARED, bool WIDE_OWN>
 __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(PagedArgs p, int split) {
@@ -521,6 +530,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(PagedArgs p, int
   else attend_part<HD, WIDE_OWN ? 4 : 1, WIDE_OWN ? 64 : 16, false>(p, blockIdx.x - split, lds, ids);
 }
 
+// Bound by the partial sums' way back: 67 MB in 13.5 us (4.9 TB/s) at 2048 rows in 16 slots, 36 MB in 9 us at 512 rows, 3-5 us
+// (a launch and two trips) where there are few rows. More wavefronts a row were slower from 512 rows on.
 // Joins the slots of a (row, head): four channels a lane, the slots dealt to the wavefronts, whose sums
 // meet in LDS. Chunks past what the row sees were not computed for it, or hold nothing of it, and are
 // not read.

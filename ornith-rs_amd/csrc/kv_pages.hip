@@ -20,6 +20,9 @@ struct CopyArgs {
   size_t run_stride;     // elements from one stretch to the next
 };
 
+// 16 bytes a lane, one piece each: 240 whole pages of 64 rows in ten layers (315 MB read, as much written) take
+// 111 us, 5.7 TB/s, the rate of a device copy of which part stays in the cache (one of 2 GiB reaches 4.9).
+// Three copies of 29 rows of one page (2.4 MB) take 3.1 us, a launch's worth.
 // grid (pieces / 256, pairs, K and V of the layers)
 __global__ __launch_bounds__(256) void kv_copy_kernel(CopyArgs a) {
   const int i = blockIdx.x * 256 + threadIdx.x;

@@ -100,6 +100,9 @@ __device__ __forceinline__ void move_to(float m_new, float& m, float& l, float& 
   m = m_new;
 }
 
+// Bound by the logits' stream: 700 rows of 248320 bf16 (348 MB) take 69-76 us, 4.6-5.0 TB/s, as a copy; four
+// tenths of its wavefronts' cycles are waits for memory, and the exponentials hide behind them. One row takes
+// 3.2 us, a launch's worth.
 // grid (runs of groups / 4, rows)
 template <bool F32>
 __global__ __launch_bounds__(256) void logprobs_sum_kernel(LogprobArgs p) {
@@ -281,6 +284,10 @@ __device__ __forceinline__ uint32_t select_best(int n, int k, Select& sh) {
   return sh.least;
 }
 
+// A chain of latencies: the sums and the groups' best values, four to six turns of the count, the best groups'
+// logits, a rank. 9.2 us for one row with twenty alternatives of 248320, 6.4 us for four rows with five of 32768
+// (f32), 19 us for 700 rows with eight, two workgroups of 1024 a compute unit. (17.6 and 32 with a selection
+// that was unrolled and cut by one bit a turn: with one workgroup the code's own way in counts.)
 // grid (rows)
 template <bool F32>
 __global__ __launch_bounds__(kFinish) void logprobs_finish_kernel(LogprobArgs p) {
