@@ -42,7 +42,8 @@ struct LogprobArgs {
   float* lse;              // [rows]
   uint32_t* top_ids;       // [rows, k]
   float* top_logprobs;     // [rows, k]
-  float4* sums;            // [rows, runs]: m, L, S, and what rounding the exponents took from L
+  float4* sums;            // [rows, runs]: m, L without its terms of 1, S, and what rounding the exponents took from L
+  float* ones;             // [rows, runs]: how many terms of L are 1 (the maximum's)
   uint32_t* best;          // [rows, groups]: order of the best value
   int64_t stride;
   int V, n_tokens, k;
@@ -91,9 +92,13 @@ struct Row {
   }
 };
 
-// (m, L, S, C) of two parts as one: S follows the reference point, e^(x - m') (x - m') = f (e^(x - m) (x - m) + e^(x - m) (m - m')).
-__device__ __forceinline__ void move_to(float m_new, float& m, float& l, float& s, float& c) {
+// The terms e^0 = 1 of L are counted apart (N): next to them the others would lose their last digits, and a
+// sure token's log probability is made of those.
+// (m, L, S, C, N) of two parts as one: S follows the reference point, e^(x - m') (x - m') = f (e^(x - m) (x - m) + e^(x - m) (m - m')).
+__device__ __forceinline__ void move_to(float m_new, float& m, float& l, float& s, float& c, float& n) {
   const float d = __builtin_elementwise_maximum(m - m_new, kFloor), f = dm_exp(d);  // (m = -inf: nothing there yet, or NaN, which stays)
+  l += n;
+  n = 0.f;
   s = f * dm_fma(l, d, s);
   l *= f;
   c *= f;
@@ -113,7 +118,7 @@ __global__ __launch_bounds__(256) void logprobs_sum_kernel(LogprobArgs p) {
   if (w >= p.runs) return;
   const R r(p, row);
   const int g_end = min(p.groups, (w + 1) * p.run);
-  float m = -DM_INF, l = 0.f, s = 0.f, c = 0.f;
+  float m = -DM_INF, l = 0.f, s = 0.f, c = 0.f, n = 0.f;
   for (int g = w * p.run; g < g_end; ++g) {
     float x[2][PER];
     const int piece = g * kGroupPieces + lane;
@@ -141,7 +146,16 @@ __global__ __launch_bounds__(256) void logprobs_sum_kernel(LogprobArgs p) {
           low = low || (r.has(t) && x[u][i] == -DM_INF);
         }
     }
-    if (best > m) move_to(best, m, l, s, c);
+    if (best > m) move_to(best, m, l, s, c, n);
+    if (best == m && __builtin_fabsf(m) < DM_INF) {  // (few groups hold the maximum so far; no distribution has an infinite one)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          n += x[u][i] == m ? 1.f : 0.f;
+          x[u][i] = x[u][i] == m ? -DM_INF : x[u][i];
+        }
+    }
     const float ref = m > -DM_INF ? m : 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -165,7 +179,11 @@ __global__ __launch_bounds__(256) void logprobs_sum_kernel(LogprobArgs p) {
   l = dm_wave_sum<64>(l);
   s = dm_wave_sum<64>(s);
   c = dm_wave_sum<64>(c);
-  if (lane == 0) p.sums[row * p.runs + w] = make_float4(m, l, s, c);
+  n = dm_wave_sum<64>(n);
+  if (lane == 0) {
+    p.sums[row * p.runs + w] = make_float4(m, l, s, c);
+    p.ones[row * p.runs + w] = n;
+  }
 }
 
 // The value that order_of made `o` of (-0 as 0, any NaN as one).
@@ -294,6 +312,7 @@ __global__ __launch_bounds__(kFinish) void logprobs_finish_kernel(LogprobArgs p)
   using R = Row<F32>;
   constexpr int PER = R::PER, SHIFT = F32 ? 0 : 16;  // (a bf16's order is in its upper half)
   __shared__ float4 red[kFinish / 64];
+  __shared__ float red_n[kFinish / 64];
   __shared__ Select sel;
   __shared__ int groups[kMaxTop], n_cands;
   __shared__ uint32_t cand_o[kCands], cand_i[kCands];
@@ -303,7 +322,11 @@ __global__ __launch_bounds__(kFinish) void logprobs_finish_kernel(LogprobArgs p)
 
   // everything that does not wait for something else is asked for first
   float4 part = make_float4(-DM_INF, 0.f, 0.f, 0.f);
-  if (tid < p.runs) part = p.sums[row * p.runs + tid];  // (runs <= the workgroup)
+  float n1 = 0.f;
+  if (tid < p.runs) {  // (runs <= the workgroup)
+    part = p.sums[row * p.runs + tid];
+    n1 = p.ones[row * p.runs + tid];
+  }
   if (p.k)
 #pragma unroll 1
     for (int i = tid; i < p.groups; i += kFinish) sel.key[i] = p.best[row * p.groups + i] >> SHIFT;
@@ -315,17 +338,25 @@ __global__ __launch_bounds__(kFinish) void logprobs_finish_kernel(LogprobArgs p)
   if (tid == 0) n_cands = 0;
   // the row's sums
   const float wm = dm_wave_max<64>(part.x);
-  if (part.x < wm) move_to(wm, part.x, part.y, part.z, part.w);
+  if (part.x < wm) move_to(wm, part.x, part.y, part.z, part.w, n1);
   part = make_float4(wm, dm_wave_sum<64>(part.y), dm_wave_sum<64>(part.z), dm_wave_sum<64>(part.w));
-  if (lane == 0) red[wave] = part;
+  n1 = dm_wave_sum<64>(n1);
+  if (lane == 0) {
+    red[wave] = part;
+    red_n[wave] = n1;
+  }
   __syncthreads();
   part = red[lane & 15];
+  n1 = red_n[lane & 15];
   const float m = dm_wave_max<16>(part.x);
-  if (part.x < m) move_to(m, part.x, part.y, part.z, part.w);
-  const float s = dm_row_sum(part.z), l = dm_fma(kLn2, dm_fma(kL2ELow, s, dm_row_sum(part.w)), dm_row_sum(part.y));
+  if (part.x < m) move_to(m, part.x, part.y, part.z, part.w, n1);
+  const float s = dm_row_sum(part.z), rest = dm_fma(kLn2, dm_fma(kL2ELow, s, dm_row_sum(part.w)), dm_row_sum(part.y));
+  n1 = dm_row_sum(n1);
+  // L = l + low, the sum and what its rounding left; ln L = ln l + low / l
+  const float l = n1 + rest, back = l - n1, low = (n1 - (l - back)) + (rest - back);
   const float ref = m > -DM_INF ? m : 0.f;
   const bool none = l == 0.f;
-  const float logl = none ? 0.f : dm_log(l);
+  const float logl = none ? 0.f : dm_log(l) + low / l;
   if (tid == 0) {
     if (p.lse) p.lse[row] = none ? -DM_INF : ref + logl;
     if (p.entropy) p.entropy[row] = none ? 0.f : logl - s / l;
@@ -464,9 +495,10 @@ extern "C" int ornith_token_logprobs(ornith_ctx* ctx, const void* d_logits, int 
   p.run = (int)std::min<int64_t>(8, std::max<int64_t>((p.groups + kFinish - 1) / kFinish, (int64_t)rows * p.groups / (32 * ctx->compute_units)));
   p.runs = (p.groups + p.run - 1) / p.run;
   void* base = nullptr;
-  if (int rc = ornith_scratch(ctx, (size_t)rows * (p.runs * sizeof(float4) + p.groups * 4) + 512, &base)) return rc;
+  if (int rc = ornith_scratch(ctx, (size_t)rows * (p.runs * (sizeof(float4) + 4) + p.groups * 4) + 768, &base)) return rc;
   ScratchCursor sc(base);
   p.sums = sc.take<float4>((size_t)rows * p.runs);
+  p.ones = sc.take<float>((size_t)rows * p.runs);
   p.best = sc.take<uint32_t>((size_t)rows * p.groups);
   const dim3 grid((p.runs + 3) / 4, rows);
   if (dtype == ORNITH_F32) hipLaunchKernelGGL(logprobs_sum_kernel<true>, grid, dim3(256), 0, ctx->stream, p);
