@@ -177,3 +177,18 @@ def test_calls_in_a_row_and_two_contexts(orn, ctx):
         _check(x, tokens, k, a)
         assert all(np.array_equal(p, q) for p, q in zip(a, b))
     other.close()
+
+
+def test_sure_tokens_keep_their_digits(orn, ctx):
+    """log p = -ln(1 + rest) with a small rest: off by 200 u of it, u = 2^-24 (an exponential 20 u with its argument's rounding, up to 140
+    additions one after another, the logarithm and the end 10), not by u of the 1 beside it."""
+    rng = np.random.default_rng(37)
+    for V in (600, 5000, 248320):
+        x = rng.standard_normal((3, V)).astype(np.float32) - np.float32(16.0 + np.log(V / 600))
+        at = rng.integers(0, V, (3, 1))
+        np.put_along_axis(x, at, np.float32(0.25), 1)
+        d = x.astype(np.float64) - 0.25
+        np.put_along_axis(d, at, -np.inf, 1)
+        rest = np.exp(d).sum(1)
+        got = _run(orn, ctx, x, orn.F32, at, 0)[0][:, 0].astype(np.float64)
+        assert (np.abs(got + np.log1p(rest)) <= 200 * 2.0 ** -24 * rest).all(), (V, got, rest)
