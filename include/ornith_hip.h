@@ -474,8 +474,8 @@ ORNITH_API int ornith_attn_prep_paged(ornith_ctx* ctx, const ornith_kv_pages* pa
 /* ornith_sdpa_decode_gated for a batch over pages: row t of sequence b sees the keys
  * [0, d_lens[b] - T + t]; a row that sees none gives zeros. out bf16 [B, T, Hq, hd] =
  * sigmoid(gate) * attention, gate in the second half of d_qg [B, T, Hq, 2*hd]; with d_qg null the
- * attention alone. scale > 0. Scores, softmax and sums are fp32, probabilities go to the matrix
- * cores as bf16: the results agree with ornith_sdpa_decode_gated's to rounding, not bit for bit.
+ * attention alone. scale > 0. Scores, softmax and sums are fp32, probabilities count to 2^-16 of
+ * themselves: the results agree with ornith_sdpa_decode_gated's to rounding, not bit for bit.
  * The sums of parts of the cache meet in the context's own memory: a call that needs more of it than
  * any before waits for the stream while it is allocated anew. */
 ORNITH_API int ornith_sdpa_paged_gated(ornith_ctx* ctx, const ornith_kv_pages* pages, int layer, const ornith_kv_batch* batch,
