@@ -1,0 +1,76 @@
+"""GPU: scores and values that are not finite in the attention over a paged KV cache, wherever its cuts fall.
+
+Keys are u, -u or -inf in one channel, queries u (u: ones and minus ones, u of that channel 1), so that a score is S, -S or -inf and a
+weight exactly 1 or, 2 S scale log2(e) > 160 binary orders below, 0."""
+import numpy as np
+import pytest
+
+import util
+from test_gpu_attn_paged import Case, _attend, _f
+
+pytestmark = pytest.mark.gpu
+
+# (query heads, KV heads, head width), lengths, new rows, shared rows: one launch; shared and own chunks; many chunks; tiles of 64 rows
+FORMS = [((4, 2, 64), [60], 1, 0), ((16, 2, 256), [100, 150], 2, 0), ((16, 2, 256), [600, 700, 650], 1, 576), ((8, 1, 128), [2500, 2000], 2, 0),
+         ((16, 2, 256), [1100, 1190, 1080], 20, 1024), ((16, 1, 64), [900, 800], 20, 0), ((16, 2, 256), [40, 33], 24, 0)]
+
+
+def _case(rng, ctx, heads, lens, T, shared, key):
+    """key(b, j): +1 or -1 for a key of sequence b (its row j) that scores S or -S, 0 for one that scores minus infinity"""
+    Hq, Hkv, hd = heads
+    c = Case(ctx, rng, lens, T, shared, 64, Hq, Hkv, hd)
+    unit = rng.choice([-1.0, 1.0], hd).astype(np.float32)
+    unit[5] = 1
+    row = {s: util.f32_to_bf16(s * (4 if hd == 256 else 8) * unit) for s in (1, -1)}
+    row[0] = np.zeros(hd, np.uint16)
+    row[0][5] = 0xff80
+    for b in range(c.B):
+        for j in range(shared if b else 0, max(lens[b], shared)): c.k[0, c.table[b, j // 64], :, j % 64] = row[key(b, j)]
+    return c, np.broadcast_to(util.f32_to_bf16(unit), (c.B, T, Hq, hd)).copy()
+
+
+def _run(orn, ctx, c, q):
+    c.upload(orn)
+    got = _f(_attend(orn, ctx, c, q, None, c.hd ** -0.5))
+    c.free()
+    return got
+
+
+@pytest.mark.parametrize("weight", [1, -1])
+@pytest.mark.parametrize("heads,lens,T,shared", FORMS)
+def test_infinite_values(orn, ctx, heads, lens, T, shared, weight):
+    """An infinite value with the weight of the row's largest score leaves its channel infinite, one whose weight underflows not
+    finite, wherever it lies; the other channels, and the rows that do not see it, are as without it."""
+    for place in sorted({0, 17, lens[-1] // 2, max(lens[-1] - T - 1, 0), lens[-1] - 1, max(shared - 1, 0)}):
+        rng = np.random.default_rng(3)
+        c, q = _case(rng, ctx, heads, lens, T, shared, lambda b, j: weight if j == place else 1)
+        last = len(lens) - 1
+        clean = _run(orn, ctx, c, q)
+        c.v[0, c.table[last, place // 64], :, place % 64, 3] = 0xff80
+        got = _run(orn, ctx, c, q)
+        for b, n in enumerate(lens):
+            for t in range(T):
+                if n - T + t >= place and (b == last or place < shared):
+                    x = got[b, t, :, 3]
+                    assert not np.isfinite(x).any(), (place, b, t)
+                    if weight == 1 or n - T + t + 1 == 1: assert (x == -np.inf).all(), (place, b, t, x)
+                    assert np.array_equal(np.delete(got[b, t], 3, -1), np.delete(clean[b, t], 3, -1)), (place, b, t)
+                else: assert np.array_equal(got[b, t], clean[b, t]), (place, b, t)
+
+
+@pytest.mark.parametrize("heads,lens,T,shared", FORMS)
+def test_infinite_values_in_parts_of_no_weight(orn, ctx, heads, lens, T, shared):
+    """The last row of every sequence alone has weight; an infinite value lies among rows of which whole chunks have none."""
+    last = len(lens) - 1
+    for place in sorted({0, 17, lens[-1] // 2, max(shared - 1, 0)}):
+        rng = np.random.default_rng(5)
+        c, q = _case(rng, ctx, heads, lens, T, shared, lambda b, j: 1 if j >= lens[b] - T else -1)
+        clean = _run(orn, ctx, c, q)
+        c.v[0, c.table[last, place // 64], :, place % 64, 3] = 0x7f80
+        got = _run(orn, ctx, c, q)
+        for b, n in enumerate(lens):
+            for t in range(T):
+                if n - T + t >= place and (b == last or place < shared):
+                    assert not np.isfinite(got[b, t, :, 3]).any(), (place, b, t)
+                    assert np.array_equal(np.delete(got[b, t], 3, -1), np.delete(clean[b, t], 3, -1)), (place, b, t)
+                else: assert np.array_equal(got[b, t], clean[b, t]), (place, b, t)
