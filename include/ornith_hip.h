@@ -476,8 +476,9 @@ ORNITH_API int ornith_attn_prep_paged(ornith_ctx* ctx, const ornith_kv_pages* pa
  * sigmoid(gate) * attention, gate in the second half of d_qg [B, T, Hq, 2*hd]; with d_qg null the
  * attention alone. scale > 0. Scores, softmax and sums are fp32, probabilities count to 2^-16 of
  * themselves: the results agree with ornith_sdpa_decode_gated's to rounding, not bit for bit.
- * A value that is not finite, at a key that a row sees, leaves the row's channel not finite whatever the
- * key's weight: infinite, or no number where the weight underflows to 0.
+ * A row all of whose scores are -inf has no distribution: its results are not numbers. A value that is
+ * not finite, at a key that a row sees, leaves the row's channel not finite whatever the key's weight:
+ * infinite, or no number where the weight underflows to 0.
  * The sums of parts of the cache meet in the context's own memory: a call that needs more of it than
  * any before waits for the stream while it is allocated anew. */
 ORNITH_API int ornith_sdpa_paged_gated(ornith_ctx* ctx, const ornith_kv_pages* pages, int layer, const ornith_kv_batch* batch,

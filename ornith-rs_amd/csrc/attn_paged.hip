@@ -159,13 +159,14 @@ __device__ __forceinline__ int least_of_rows(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-// The last step of four channels of a row: values / sum (a row that sees nothing has no sum: zeros), the gate, one rounding.
+// The last step of four channels of a row: values / sum (zeros for a row that sees no key; one whose scores are all
+// minus infinity has the sum 0, and no number comes out), the gate, one rounding.
 template <int HD>
-__device__ __forceinline__ void store_result(const PagedArgs& p, size_t row_head, int ch, const f32x4_t& o, float l) {
-  const float inv = l != 0.f ? 1.0f / l : 0.f;
+__device__ __forceinline__ void store_result(const PagedArgs& p, size_t row_head, int ch, const f32x4_t& o, float l, bool sees) {
+  const float inv = 1.0f / l;
   float y[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = l != 0.f ? o[e] * inv : 0.f;
+  for (int e = 0; e < 4; ++e) y[e] = sees ? o[e] * inv : 0.f;
   if (p.qg) {
     const u32x2_t gw = *reinterpret_cast<const u32x2_t*>(p.qg + row_head * 2 * HD + HD + ch);
 #pragma unroll
@@ -507,7 +508,7 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
   constexpr int NT = KW > 1 ? NC / KW : NC;
   if (finishes) {
 #pragma unroll
-    for (int u = 0; u < NT; ++u) store_result<HD>(p, row_head, 16 * (t_lo + u) + 4 * lg, o[u], vis > 0 ? l_i : 0.f);
+    for (int u = 0; u < NT; ++u) store_result<HD>(p, row_head, 16 * (t_lo + u) + 4 * lg, o[u], l_i, vis > 0);
     return;
   }
   const size_t at = (size_t)((SHARED ? 0 : p.chunks[0]) + chunk) * p.b.B * p.T * p.Hq + row_head;
@@ -608,7 +609,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedArgs p) {
       o[3] = dm_fma(x.w, w, o[3]);
     }
   }
-  store_result<HD>(p, row_head, ch, o, l);
+  store_result<HD>(p, row_head, ch, o, l, vis > 0);
 }
 
 template <int HD>

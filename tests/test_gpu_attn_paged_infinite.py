@@ -36,6 +36,38 @@ def _run(orn, ctx, c, q):
     return got
 
 
+@pytest.mark.parametrize("heads,lens,T,shared", FORMS)
+def test_every_score_is_minus_infinity(orn, ctx, heads, lens, T, shared):
+    rng = np.random.default_rng(1)
+    c, q = _case(rng, ctx, heads, lens, T, shared, lambda b, j: 0)
+    got = _run(orn, ctx, c, q)
+    for b, n in enumerate(lens):
+        for t in range(T):
+            if n - T + t < 0: assert (got[b, t] == 0).all()
+            else: assert np.isnan(got[b, t]).all(), (b, t)
+
+
+@pytest.mark.parametrize("heads,lens,T,shared", FORMS)
+def test_parts_of_minus_infinity_scores(orn, ctx, heads, lens, T, shared):
+    """Everything but the last rows of the last sequence and one early row of the first: whole chunks and wavefronts have no finite score."""
+    rng = np.random.default_rng(2)
+    last, one = len(lens) - 1, min(lens[0], max(shared, lens[0])) // 3
+    alive = lambda b, j: 1 if (b == last and j >= lens[b] - T - 2 and j >= shared) or (b == 0 and j == one) else 0
+    c, q = _case(rng, ctx, heads, lens, T, shared, alive)
+    got = _run(orn, ctx, c, q)
+    for b, n in enumerate(lens):
+        v = c.rows(c.v, b, n)
+        for t in range(T):
+            seen = [j for j in range(max(n - T + t + 1, 0)) if alive(0 if j < shared else b, j)]
+            for h in range(heads[0]):
+                if not seen and n - T + t >= 0: assert np.isnan(got[b, t, h]).all(), (b, t, h)
+                elif seen:
+                    vv = v[h // (heads[0] // heads[1])][seen]
+                    want = vv.mean(0)
+                    # one reciprocal, sums of len(seen) terms, the rounding to bf16
+                    assert (np.abs(got[b, t, h] - want) <= 2.0 ** -8 * np.abs(want) + (len(seen) + 4) * 2.0 ** -24 * np.abs(vv).mean(0)).all(), (b, t, h)
+
+
 @pytest.mark.parametrize("weight", [1, -1])
 @pytest.mark.parametrize("heads,lens,T,shared", FORMS)
 def test_infinite_values(orn, ctx, heads, lens, T, shared, weight):
