@@ -413,7 +413,13 @@ class KvBatch:
 
 
 def _ids(a):
-    """A list of page ids as (number, C array); the array keeps its own copy alive."""
+    """A list of page ids as (number, C array); the array keeps its own copy alive. Only whole numbers of 32 bits: nothing is wrapped or cut."""
+    a = np.asarray(a)
+    if a.dtype != np.uint32 and a.size:
+        if a.dtype.kind not in "iu":
+            raise TypeError(f"page ids are whole numbers, not {a.dtype}")
+        if a.min() < 0 or a.max() > 0xFFFFFFFF:
+            raise OverflowError("page ids have 32 bits")
     a = np.array(a, dtype=np.uint32, order="C").reshape(-1)
     return a.size, (C.c_uint32 * a.size).from_buffer(a) if a.size else None
 

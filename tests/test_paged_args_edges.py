@@ -1,0 +1,26 @@
+"""CPU: the ends of the ranges of what the calls over paged KV caches and the token scores take."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from test_paged_args import _batch, _copy, _pages, _refused, _score, _sdpa
+
+
+@pytest.mark.parametrize("ids", [[1 << 32], [-1], [1.0], [True], ["1"], np.array([(1 << 32) + 1]), np.array([-1]), np.array([1 << 32], np.uint64), np.array([2.5])])
+def test_page_ids_of_other_types(orn, ids):
+    """A number that is no 32-bit page id is refused; it is not wrapped or cut to one."""
+    ctx = orn.Ctx.__new__(orn.Ctx)
+    ctx.h = None
+    for call in (lambda: ctx.kv_pages_copy(_pages(orn), ids, [3], 1), lambda: ctx.kv_pages_copy(_pages(orn), [3], ids, 1),
+                 lambda: ctx.kv_pages_load(_pages(orn), 0, _pages(orn).keep[0][0], _pages(orn).keep[0][0], 64, 0, 1, ids, 0),
+                 lambda: ctx.kv_pages_store(_pages(orn), 0, _pages(orn).keep[0][0], _pages(orn).keep[0][0], 64, 0, 1, ids, 0)):
+        with pytest.raises((TypeError, OverflowError), match="page ids"): call()
+
+
+@pytest.mark.parametrize("dtype", [np.int8, np.uint8, np.int32, np.uint32, np.int64, np.uint64])
+def test_page_ids_of_whole_types(orn, dtype):
+    n, ids = orn._ids(np.array([[0, 7], [100, 3]], dtype)[:, ::-1])
+    assert n == 4 and list(ids) == [7, 0, 3, 100]
+    assert list(orn._ids(range(3))[1]) == [0, 1, 2] and orn._ids([]) == (0, None) and orn._ids(np.zeros(0)) == (0, None)
+    assert list(orn._ids([np.uint32(5), np.int64(2 ** 32 - 1)])[1]) == [5, 2 ** 32 - 1]
