@@ -546,7 +546,7 @@ ORNITH_API int ornith_argmax_rows(ornith_ctx* ctx, const void* d_logits, int row
 /* Log probabilities of given tokens under rows of logits (bf16 or f32 by dtype, row r at
  * d_logits + r * row_stride elements, no alignment beyond the element's), for scoring a text or
  * ranking continuations; no counterpart in the reference. Natural logarithms, all outputs fp32:
- *   d_logprobs [rows, n_tokens]  of d_tokens [rows, n_tokens]; n_tokens may be 0 (both may be null)
+ *   d_logprobs [rows, n_tokens]  of d_tokens [rows, n_tokens]; n_tokens: 0 (both may be null) to 2^30
  *   d_entropy, d_lse [rows]      may be null
  *   d_top_ids, d_top_logprobs [rows, k]  the k <= 32 most probable tokens, falling; equal logits by
  *                                the lower id; k may be 0 (both may be null)

@@ -470,6 +470,7 @@ extern "C" int ornith_token_logprobs(ornith_ctx* ctx, const void* d_logits, int 
   ORN_REQUIRE(dtype == ORNITH_F32 || dtype == ORNITH_BF16, "token_logprobs: dtype %d", dtype);
   ORN_REQUIRE(rows >= 1 && rows <= 65535 && V >= 1 && row_stride >= V, "token_logprobs: rows=%d V=%d row_stride=%lld", rows, V, (long long)row_stride);
   ORN_REQUIRE(n_tokens >= 0 && (n_tokens == 0 || (d_tokens && d_logprobs)), "token_logprobs: %d tokens a row without their arrays", n_tokens);
+  ORN_REQUIRE(n_tokens <= 1 << 30, "token_logprobs: %d tokens a row (at most 2^30)", n_tokens);  // (their numbers grow by a workgroup's threads)
   ORN_REQUIRE(k >= 0 && k <= kMaxTop && k <= V, "token_logprobs: %d alternatives of %d tokens (at most %d)", k, V, kMaxTop);
   ORN_REQUIRE(k == 0 || (d_top_ids && d_top_logprobs), "token_logprobs: alternatives without their arrays");
   ORN_REQUIRE(((uintptr_t)d_logits & (dtype == ORNITH_F32 ? 3 : 1)) == 0, "token_logprobs: misaligned logits");

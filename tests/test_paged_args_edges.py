@@ -24,3 +24,10 @@ def test_page_ids_of_whole_types(orn, dtype):
     assert n == 4 and list(ids) == [7, 0, 3, 100]
     assert list(orn._ids(range(3))[1]) == [0, 1, 2] and orn._ids([]) == (0, None) and orn._ids(np.zeros(0)) == (0, None)
     assert list(orn._ids([np.uint32(5), np.int64(2 ** 32 - 1)])[1]) == [5, 2 ** 32 - 1]
+
+
+def test_more_tokens_a_row_than_can_be_counted(orn):
+    """The finishing threads step through a row's tokens by 1024: the number of the next one stays below 2^31."""
+    _refused(orn, _score(orn, n=(1 << 30) + 1), "1073741825 tokens a row (at most 2^30)")
+    _refused(orn, _score(orn, n=2 ** 31 - 1), "2147483647 tokens a row")
+    _refused(orn, _score(orn, n=1 << 30), "null context")
