@@ -711,7 +711,8 @@ int ornith_sdpa_paged_gated(ornith_ctx* ctx, const ornith_kv_pages* pages, int l
   if (int rc = rows_check(pages, batch, layer, T, Hq, "sdpa_paged")) return rc;
   ORN_REQUIRE(d_q_rot && d_out, "sdpa_paged: null argument");
   ORN_REQUIRE((((uintptr_t)d_q_rot | (uintptr_t)d_qg | (uintptr_t)d_out) & 15) == 0, "sdpa_paged: operands must be 16-byte aligned");
-  ORN_REQUIRE(scale > 0.f && scale < DM_INF, "sdpa_paged: scale %g", scale);
+  const float c2 = scale * 1.44269504088896341f;
+  ORN_REQUIRE(scale > 0.f && c2 < DM_INF, "sdpa_paged: scale %g", scale);
   ORN_REQUIRE(ctx, "sdpa_paged: null context");
   const OrnDevice on(ctx);
   PagedArgs a{};
@@ -723,7 +724,7 @@ int ornith_sdpa_paged_gated(ornith_ctx* ctx, const ornith_kv_pages* pages, int l
   a.T = T;
   a.Hq = Hq;
   a.shared = batch->shared_rows;
-  a.c2 = scale * 1.44269504088896341f;
+  a.c2 = c2;
   switch (pages->hd) {
     case 64: return attend<64>(ctx, a, batch->max_rows);
     case 128: return attend<128>(ctx, a, batch->max_rows);

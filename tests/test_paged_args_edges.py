@@ -31,3 +31,10 @@ def test_more_tokens_a_row_than_can_be_counted(orn):
     _refused(orn, _score(orn, n=(1 << 30) + 1), "1073741825 tokens a row (at most 2^30)")
     _refused(orn, _score(orn, n=2 ** 31 - 1), "2147483647 tokens a row")
     _refused(orn, _score(orn, n=1 << 30), "null context")
+
+
+@pytest.mark.parametrize("scale", [3.4e38, 2.4e38])
+def test_attention_scale_past_its_binary_logarithm(orn, scale):
+    """Scores are counted in binary orders, scale log2(e) of them a unit: a scale whose product is infinite would make 0 infinity of a row's best score."""
+    _refused(orn, _sdpa(orn, _pages(orn), _batch(orn), scale=scale), "scale")
+    _refused(orn, _sdpa(orn, _pages(orn), _batch(orn), scale=2.3e38), "null context")
