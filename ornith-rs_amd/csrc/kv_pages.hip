@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void kv_move_kernel(MoveArgs a) {
 // A set of page ids that says whether one was in it already; empty again when it goes.
 class Seen {
  public:
-  explicit Seen(int n_pages) : bits_((size_t)(n_pages + 63) / 64) {}
+  explicit Seen(int n_pages) : bits_(((size_t)n_pages + 63) / 64) {}
   bool has(uint32_t id) const { return bits_[id >> 6] >> (id & 63) & 1; }
   bool add(uint32_t id) {
     const bool was = has(id);

@@ -38,3 +38,14 @@ def test_attention_scale_past_its_binary_logarithm(orn, scale):
     """Scores are counted in binary orders, scale log2(e) of them a unit: a scale whose product is infinite would make 0 infinity of a row's best score."""
     _refused(orn, _sdpa(orn, _pages(orn), _batch(orn), scale=scale), "scale")
     _refused(orn, _sdpa(orn, _pages(orn), _batch(orn), scale=2.3e38), "null context")
+
+
+def test_as_many_pages_as_an_int_counts(orn):
+    """The set of pages that a copy or a load looks through is sized in 64 bits: no exception leaves a call."""
+    most = 2 ** 31 - 1
+    pages = _pages(orn, n_pages=most)
+    _refused(orn, _copy(orn, pages, [0, most - 1], [most - 2, 5]), "null context")
+    _refused(orn, _copy(orn, pages, [0, most - 1], [7, most - 1]), "read and written")
+    _refused(orn, _copy(orn, pages, [0], [most]), "of 2147483647")
+    ids = np.array([most - 1, most - 1], np.uint32)
+    _refused(orn, orn.lib().ornith_kv_pages_load(None, C.byref(pages.s), 0, C.c_void_p(0x1000), C.c_void_p(0x1000), 100, 0, 70, ids.ctypes.data_as(C.c_void_p), 2, 10), "twice")
