@@ -688,6 +688,11 @@ ORNITH_API int ornith_caches_create(ornith_model* m, int capacity, int max_windo
 ORNITH_API int ornith_caches_reserve(ornith_caches* c, int rows);
 ORNITH_API int ornith_caches_set_growable(ornith_caches* c, int growable);
 ORNITH_API int ornith_caches_capacity(const ornith_caches* c, int* capacity_out);
+/* Decoder layer `layer`'s K and V (bf16 [Hkv, capacity, hd], rows [0, offset) held) in a full-attention
+ * layer, to take a prompt that the model has run into pages (ornith_kv_pool_load, ornith_kv_pages_load)
+ * or to look at it; an error in a gated-delta layer. Valid until the caches grow or are destroyed; of the
+ * model's context, whose stream orders a call of the same context behind the forwards before it. */
+ORNITH_API int ornith_caches_layer_kv(const ornith_caches* c, int layer, const void** d_k_out, const void** d_v_out);
 ORNITH_API int ornith_caches_reset(ornith_caches* c);
 ORNITH_API int ornith_caches_destroy(ornith_caches* c);
 ORNITH_API int ornith_caches_offset(const ornith_caches* c, int* offset_out);

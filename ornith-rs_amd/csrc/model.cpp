@@ -436,6 +436,15 @@ int ornith_caches_capacity(const ornith_caches* cc, int* capacity_out) {
   return ORNITH_OK;
 }
 
+int ornith_caches_layer_kv(const ornith_caches* cc, int layer, const void** d_k_out, const void** d_v_out) {
+  ORN_REQUIRE(cc && d_k_out && d_v_out, "caches_layer_kv: null argument");
+  ORN_REQUIRE(layer >= 0 && layer < (int)cc->layers.size(), "caches_layer_kv: layer %d of %zu", layer, cc->layers.size());
+  ORN_REQUIRE(!cc->m->layers[layer].linear, "caches_layer_kv: layer %d is a gated-delta layer, it has no K and V", layer);
+  *d_k_out = cc->layers[layer].k;
+  *d_v_out = cc->layers[layer].v;
+  return ORNITH_OK;
+}
+
 int ornith_caches_create(ornith_model* m, int capacity, int max_window, ornith_caches** out) {
   ORN_REQUIRE(m && out, "caches_create: null argument");
   ORN_REQUIRE(capacity >= 1 && max_window >= 1 && max_window <= kMaxRows,

@@ -218,6 +218,13 @@ def quant_config_load(model_dir, path):
     return g.value, b.value, m.value
 
 
+class DeviceView:
+    """Device memory that something else owns."""
+
+    def __init__(self):
+        self.ptr = C.c_void_p()
+
+
 class Caches:
     def __init__(self, model, capacity, max_window):
         self.model = model
@@ -247,6 +254,12 @@ class Caches:
         o = C.c_int()
         _check(lib().ornith_caches_offset(self.h, C.byref(o)), "caches_offset")
         return o.value
+
+    def layer_kv(self, layer):
+        """A full-attention layer's (k, v), bf16 [Hkv, capacity, hd], as the calls over buffers take them; valid until the caches grow or close."""
+        k, v = DeviceView(), DeviceView()
+        _check(lib().ornith_caches_layer_kv(self.h, layer, C.byref(k.ptr), C.byref(v.ptr)), "caches_layer_kv")
+        return k, v
 
     def close(self):
         if self.h:
