@@ -475,7 +475,11 @@ ORNITH_API int ornith_attn_prep_paged(ornith_ctx* ctx, const ornith_kv_pages* pa
  * [0, d_lens[b] - T + t]; a row that sees none gives zeros. out bf16 [B, T, Hq, hd] =
  * sigmoid(gate) * attention, gate in the second half of d_qg [B, T, Hq, 2*hd]; with d_qg null the
  * attention alone. scale > 0. Scores, softmax and sums are fp32, probabilities count to 2^-16 of
- * themselves: the results agree with ornith_sdpa_decode_gated's to rounding, not bit for bit.
+ * themselves: the results agree with ornith_sdpa_decode_gated's to rounding, not bit for bit. Where a
+ * row's keys are cut follows from B, T, Hq, shared_rows and max_rows, and the order of its sums with
+ * it: the same call gives the same bits, but a row among other rows, or in another batch, not always those
+ * that it gives alone (ornith_sdpa_decode_gated's rows do). A program that compares drafts with steps
+ * of one token bit for bit takes that one.
  * A row all of whose scores are -inf has no distribution: its results are not numbers. A value that is
  * not finite, at a key that a row sees, leaves the row's channel not finite whatever the key's weight:
  * infinite, or no number where the weight underflows to 0.
