@@ -587,27 +587,25 @@ __global__ __launch_bounds__(64 * kJoinWaves) void join_kernel(PagedArgs p) {
       for (int e = 0; e < 4; ++e) o[e] = dm_fma(x[u][e], w, o[e] * a);
     }
   }
-  if constexpr (PARTS > 1) {
-    so[part][ch / 4] = make_float4(o[0], o[1], o[2], o[3]);
-    if (ch == 0) sml[part] = make_float2(m, l);
-    __syncthreads();
-    if (part) return;
-    float mt = -DM_INF;
+  so[part][ch / 4] = make_float4(o[0], o[1], o[2], o[3]);
+  if (ch == 0) sml[part] = make_float2(m, l);
+  __syncthreads();
+  if (part) return;
+  float mt = -DM_INF;
 #pragma unroll
-    for (int q = 0; q < PARTS; ++q) mt = fmaxf(mt, sml[q].x);
-    l = 0.f;
-    o = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int q = 0; q < PARTS; ++q) mt = fmaxf(mt, sml[q].x);
+  l = 0.f;
+  o = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < PARTS; ++q) {
-      const float2 v = sml[q];
-      const float4 x = so[q][ch / 4];
-      const float w = v.x > -DM_INF ? __builtin_amdgcn_exp2f((v.x - mt) * p.c2) : v.y != v.y ? 1.f : 0.f;
-      l = dm_fma(v.y, w, l);
-      o[0] = dm_fma(x.x, w, o[0]);
-      o[1] = dm_fma(x.y, w, o[1]);
-      o[2] = dm_fma(x.z, w, o[2]);
-      o[3] = dm_fma(x.w, w, o[3]);
-    }
+  for (int q = 0; q < PARTS; ++q) {
+    const float2 v = sml[q];
+    const float4 x = so[q][ch / 4];
+    const float w = v.x > -DM_INF ? __builtin_amdgcn_exp2f((v.x - mt) * p.c2) : v.y != v.y ? 1.f : 0.f;
+    l = dm_fma(v.y, w, l);
+    o[0] = dm_fma(x.x, w, o[0]);
+    o[1] = dm_fma(x.y, w, o[1]);
+    o[2] = dm_fma(x.z, w, o[2]);
+    o[3] = dm_fma(x.w, w, o[3]);
   }
   store_result<HD>(p, row_head, ch, o, l, vis > 0);
 }

@@ -32,8 +32,6 @@ constexpr int kMaxV = (kGroups * kGroupPieces - 1) * 4;  // logits a row: what f
 constexpr float kL2E = 1.44269502162933349609375f, kL2ELow = 1.925963033500e-8f, kLn2 = 0.693147180559945309f;
 constexpr float kFloor = -200.f;             // e^kFloor is 0 in fp32: differences stop there, so that -inf makes no NaN
 
-typedef unsigned int u32x4_t __attribute__((ext_vector_type(4)));
-
 struct LogprobArgs {
   const void* x;
   const uint32_t* tokens;  // [rows, n_tokens]
