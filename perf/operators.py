@@ -9,7 +9,9 @@ The operators a program needs that keeps the prompt's KV cache once and decodes 
 
 Shapes are those of the full-attention layers of the model this library serves (16 query heads on 2
 KV heads of 256, ten such layers, a vocabulary of 248320 and a draft vocabulary of 32768), or generic.
-Where `own` is false everything is elementary torch arithmetic.
+Where `own` is false everything is elementary torch arithmetic. Where it is true the calls run on the stream of the library's own
+context, which is not ordered with torch's: `prepare` waits until torch has made the inputs, and who reads a pass's outputs, times it or
+changes its inputs waits for the whole device first (torch.cuda.synchronize()).
 """
 import ctypes as C
 import importlib
@@ -136,6 +138,8 @@ def prepare(case, seed):
     s, g = _State(case), torch.Generator(device="cuda")
     g.manual_seed(seed)
     {"logprobs": _prep_logprobs, "copy": _prep_copy, "append": _prep_append, "attention": _prep_attention}[case["op"]](s, case, g)
+    if own:
+        torch.cuda.synchronize()  # (another stream than torch's reads them)
     return s
 
 
