@@ -41,8 +41,8 @@ struct AppendArgs {
 // One wavefront a (head, row): inv = rsqrt(mean x^2 + eps), x inv w, and channel e turned against e + half by
 // the position's angle. A chain of latencies (length, page, row; norm across the lanes), with no work to
 // speak of: 3.2 us at 8 rows of 20 heads of 256 (160 KB), 4.5 us at 256 rows (5.2 MB; a copy of it takes
-// 1.1 us), where one launch after another takes 3.9 us either way. The row itself and the norm's weights
-// do not wait for the page: that took 0.6 us off.
+// 1.1 us), where one launch after another takes 3.9-4.9 us either way, by the machine. The row itself and the
+// norm's weights do not wait for the page: that took 0.6 us off.
 // The norm and the rotation stay fp32 and are rounded once, on the store. (ornith_attn_prep rounds the
 // norm's two products to bf16 as the reference's rms_norm does; nothing here is compared bit for bit with
 // a contiguous cache's rows, so the values keep what they have.)
@@ -182,7 +182,8 @@ __device__ __forceinline__ void store_result(const PagedArgs& p, size_t row_head
 //   RW = 4, BK = 64  four wavefronts of 16 query rows share a block of 64 keys
 //   RW = 1, BK = 16  16 query rows; every wavefront has a block of 16 keys of its own in turn, and their
 //                    sums meet at the end (few rows: what counts is how much is in flight)
-// Both take 64 KB of LDS at a head width of 256, two workgroups a compute unit.
+// Both take 64 KB of LDS at a head width of 256 (the second one 512 bytes more, where its sums meet), two
+// workgroups a compute unit.
 //
 // Both products run transposed, so that a lane owns a query row from the scores to the output and the
 // probabilities never leave the registers:
@@ -524,13 +525,17 @@ constexpr int attend_lds() {
 }
 
 // What it measured, 16 query heads on 2 KV heads of 256, shared keys / own keys a sequence, both forms in one launch:
-//   2048 rows (64 sequences of 4 tokens x 8 heads), 32768 / 512   168-219 us by the card's clock, 640-830 TFLOP/s
-//   512 rows (16 x 4 x 8), 16256 / 77                             34 us, 500 TFLOP/s
+//   2048 rows (64 sequences of 4 tokens x 8 heads), 32768 / 512   202-242 us by the card's clock, 570-690 TFLOP/s
+//   512 rows (16 x 4 x 8), 16256 / 77                             38 us, 450 TFLOP/s
 //   64 rows (8 x 1 x 8), 6592 / 200                               13-14 us, where a copy of its 16 MB takes 3.3
-// Wide: the matrix cores are busy a third of the time, LDS a third (V's transposing reads run at half the
-// rate of K's), half of the wavefronts' cycles are waits at the two barriers a block. With the fetches
-// taken out 185 us became 140, with V's reads 152, the softmax was within the noise. Larger tiles (128 rows, each
+//   8 rows a sequence, nothing shared: one of 32768 keys 14-15 us, 4.5 TB/s; 8 of 4000-8000 19 us, 64 of 750-1500 25 us, 5 TB/s and more
+// Wide: the matrix cores are busy for 47 % of the time (38 % at 512 rows), LDS a third (V's transposing reads run at half the
+// rate of K's), 38 % of the wavefronts' cycles are waits, most of them at the four barriers a block: K's tile and V's have
+// arrived, K's and V's may be written again. With one part of each probability alone, 185 us became 140 with the fetches
+// taken out and 152 with V's reads; the softmax was within the noise. Larger tiles (128 rows, each
 // fragment of K and V for two products) were 188-195 us with twice the partial sums, 32 x 32 products slower.
+// At a width of 256 the wide forms have 256 registers, and 29 and 56 of them in scratch memory: around and in
+// the loop of blocks with masks, none in the loop of full blocks.
 // Narrow: a chain of trips to memory, table, keys, values a turn; a workgroup has as much in flight as LDS holds.
 // Workgroups below `split` have chunks of the shared part, the others of the sequences' own.
 template <int HD, bool WIDE_SHARED, bool WIDE_OWN>
@@ -541,8 +546,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void attend_kernel(PagedArgs p, int
   else attend_part<HD, WIDE_OWN ? 4 : 1, WIDE_OWN ? 64 : 16, false>(p, blockIdx.x - split, lds, ids);
 }
 
-// Bound by the partial sums' way back: 67 MB in 13.5 us (4.9 TB/s) at 2048 rows in 16 slots, 36 MB in 9 us at 512 rows, 3-5 us
-// (a launch and two trips) where there are few rows. More wavefronts a row were slower from 512 rows on.
+// 42 MB in 13.5 us (3.1 TB/s) at 2048 rows in 10 slots, 35 MB in 9 us (3.9 TB/s) at 512 rows in 33, 4 us (a launch and two
+// trips) where there are few rows, 10 us for 8 rows in 171 slots. A chain of trips: lengths, then a wavefront's share of the
+// slots at once, then LDS; at 10 slots a wavefront has two or three loads in flight, and 56 % of the wavefronts' cycles
+// are waits. More wavefronts a row were slower from 512 rows on.
 // Joins the slots of a (row, head): four channels a lane, the slots dealt to the wavefronts, whose sums
 // meet in LDS. Chunks past what the row sees were not computed for it, or hold nothing of it, and are
 // not read. A slot of weight 0 is added like the others: a value in it that is not finite makes no number
@@ -615,19 +622,24 @@ int attend(ornith_ctx* ctx, PagedArgs a, int max_rows) {
   const int own_rows = a.T * (a.Hq / a.l.Hkv), shared_rows = a.b.B * own_rows;
   // Wide from more than 128 rows: below, the tiles of 16 rows read their keys out of the die's cache often
   // enough, and their chunks are longer, so that less goes through memory. Both launches, us, narrow / wide,
-  // 2 KV heads of 256: 64 rows at 2000 keys 11.3 / 13.3, at 6621 17.1 / 16.8; 128 rows at 2000 12.9 / 14.8, at
-  // 6621 19.8 / 21.4, at 16300 26.8 / 32.1; 192 rows at 6621 23.4 / 25.3, at 16300 36.4 / 33.8; 256 rows at 6621
-  // 26.4 / 27.8, at 16300 34.9 / 34.4; 512 rows at 16300 54.8 / 43.
+  // at 2000 / 6600 / 16300 keys: 2 KV heads of 256, 64 rows 11.2 / 13.4, 16.2 / 17.6, 22.6 / 23.4; 128 rows 11.8 / 14.6, 19.7 / 21.8,
+  // 26.1 / 31.9; 192 rows 15.0 / 15.8, 23.0 / 25.5, 36.0 / 34.2; 256 rows 16.4 / 17.7, 25.4 / 27.2, 33.6 / 35.0; 512 rows
+  // 21.6 / 22.3, 30.4 / 29.9, 52.3 / 43.4. 8 KV heads of 128: 128 rows 14.5 / 16.1, 20.1 / 22.3; 192 rows 19.8 / 20.1, 26.0 / 25.7; 256 rows
+  // 21.0 / 22.4, 30.1 / 28.8. 2 KV heads of 128: 192 rows 10.8 / 11.5, 14.4 / 18.0; 384 rows 13.5 / 13.3, 19.4 / 21.1. One of 64: 256 rows
+  // 8.7 / 9.2, 10.4 / 10.7, 512 rows 10.0 / 10.2, 12.1 / 14.3: few heads, or narrow ones, could stay narrow for longer.
   const bool wide[2] = {shared_rows > 128, own_rows > 128};
   int64_t grid[2];
   const int keys[2] = {a.shared, max_rows - a.shared}, rows[2] = {shared_rows, own_rows}, seqs[2] = {1, a.b.B};
   for (int part = 0; part < 2; ++part) {
     // chunks: two workgroups for every compute unit (both launches, us, one / one and a half / two / three a
-    // unit: 512 rows at 16300 keys 44.3 / 41.7 / 43.5 / 48.6, 2048 at 32768 268 / 236 / 186 / 217); whole blocks of
+    // unit: 2 KV heads of 256, 512 rows at 16300 keys 44.6 / 44.5 / 46.7 / 51.4, 2048 at 32768 325 / 260 / 217 / 260; 8 of 128, 1024 rows at 8200
+    // 100 / 85 / 76 / 81; one of 64, 2048 rows at 16300 36 / 35.4 / 32.1 / 33; but 64 rows of 2 of 256 at 6600 13.6 / 17 / 16.9 / 17: with one
+    // each, a unit is done once); whole blocks of
     // 64 (a chunk that begins inside a page touches one page more than it has). None is shorter than 128 keys,
     // 192 in the narrow form: with more of them the sums that go through memory cost more than the keys'
-    // reads gain (at least 64 / 128 / 192 / 256 keys: wide, 64 rows at 6600 keys, 20.8 / 16.7 / 17.7 / 17.4; narrow, 32
-    // rows of 8 KV heads of 128 at 2300 keys, 13.8 / 12.3 / 10.8 / 10.9, 32 of 2 of 256 at 1000 keys, - / 10.5 / 10.6 / 11.3).
+    // reads gain (at least 64 / 128 / 192 / 256 keys, us: wide, 512 rows of 2 KV heads of 256 at 2000 keys 29.3 / 21.2 / 21.2 / 21.9, 256
+    // rows 22.9 / 17.7 / 17.4 / 18.1; narrow, 32 rows of 8 of 128 at 2000 12.4 / 10.3 / 9.7 / 9.6, 32 of 2 of 256 at 1000 10 / 10.1 / 10.5 / 10.8,
+    // 64 of 2 of 256 at 6600 18.2 / 18.2 / 17.1 / 13.8, 64 of one of 64 at 6600 9.8 / 8.7 / 8.9 / 8.9).
     const int tile = wide[part] ? 64 : 16, most = ((kChunkPages - 1) << a.l.shift) / 64 * 64;
     const int64_t tiles = (rows[part] + tile - 1) / tile, pairs = (int64_t)seqs[part] * a.l.Hkv;
     const int64_t want = std::max<int64_t>(1, (2 * ctx->compute_units + tiles * pairs - 1) / (tiles * pairs));

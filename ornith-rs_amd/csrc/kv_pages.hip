@@ -42,6 +42,8 @@ struct MoveArgs {
   int cap, row0, at, rows, row_pieces;  // cache rows [row0, row0 + rows) <-> rows [at, ..) of the pages ids[0], ids[1], ...
 };
 
+// 16 bytes a lane: 6621 rows of 2 KV heads of 256 (13.6 MB read, as much written) take 3.7-5 us, 5.4 TB/s and more (out
+// of the cache in part), 64 rows 2.4 us, a launch's worth.
 // grid (rows x pieces / 256, Hkv, 2)
 template <bool LOAD>
 __global__ __launch_bounds__(256) void kv_move_kernel(MoveArgs a) {

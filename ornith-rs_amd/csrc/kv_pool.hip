@@ -1,7 +1,9 @@
 // The pool of a paged KV cache: which sequence holds which page, who shares it, what is free. All of
 // that is host bookkeeping (a few integers a token); the device sees page copies and, when a batch is
-// asked for, one launch that writes its tables. Page ids and lengths reach the device in launch
+// asked for, a launch or two that write its tables. Page ids and lengths reach the device in launch
 // arguments, so no call waits for the stream and no host buffer has to outlive one.
+// Either launch takes 2.0-2.7 us, for 8 sequences of 104 pages as for 64: a step's extension and descriptor together,
+// through the Python binding, 7.3 us for 8 sequences and 13 us for 64.
 #include "kv_pages.h"
 
 #include <algorithm>
