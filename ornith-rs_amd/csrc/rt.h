@@ -105,12 +105,15 @@ class OrnDevice {
 // Records the message for ornith_last_error() and returns `code`.
 int ornith_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 
+// (A failure is told once: left in the runtime, it would be taken for one of the next launch.)
 #define ORN_HIP(expr)                                                                   \
   do {                                                                                  \
     hipError_t e__ = (expr);                                                            \
-    if (e__ != hipSuccess)                                                              \
+    if (e__ != hipSuccess) {                                                            \
+      (void)hipGetLastError();                                                          \
       return ornith_fail(ORNITH_ERR_HIP, "%s failed: %s (%s:%d)", #expr,                \
                          hipGetErrorString(e__), __FILE__, __LINE__);                   \
+    }                                                                                   \
   } while (0)
 
 #define ORN_REQUIRE(cond, ...)                                  \
