@@ -159,14 +159,14 @@ __device__ __forceinline__ int least_of_rows(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-// The last step of four channels of a row: values / sum (zeros for a row that sees no key; one whose scores are all
-// minus infinity has the sum 0, and no number comes out), the gate, one rounding.
+// The last step of four channels of a row: values / sum, the gate, one rounding. Zeros for a row that sees no key, whatever
+// its gate; one whose scores are all minus infinity has the sum 0, and no number comes out.
 template <int HD>
 __device__ __forceinline__ void store_result(const PagedArgs& p, size_t row_head, int ch, const f32x4_t& o, float l, bool sees) {
   const float inv = 1.0f / l;
   float y[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = sees ? o[e] * inv : 0.f;
+  for (int e = 0; e < 4; ++e) y[e] = o[e] * inv;
   if (p.qg) {
     const u32x2_t gw = *reinterpret_cast<const u32x2_t*>(p.qg + row_head * 2 * HD + HD + ch);
 #pragma unroll
@@ -175,7 +175,7 @@ __device__ __forceinline__ void store_result(const PagedArgs& p, size_t row_head
       y[e] *= __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-g * 1.44269504088896341f));
     }
   }
-  *reinterpret_cast<u32x2_t*>(p.out + row_head * HD + ch) = u32x2_t{dm_f2bf2(y[0], y[1]), dm_f2bf2(y[2], y[3])};
+  *reinterpret_cast<u32x2_t*>(p.out + row_head * HD + ch) = sees ? u32x2_t{dm_f2bf2(y[0], y[1]), dm_f2bf2(y[2], y[3])} : u32x2_t{0, 0};
 }
 
 // A workgroup of four wavefronts works in one of two forms:

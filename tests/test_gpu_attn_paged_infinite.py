@@ -106,3 +106,21 @@ def test_infinite_values_in_parts_of_no_weight(orn, ctx, heads, lens, T, shared)
                     assert not np.isfinite(got[b, t, :, 3]).any(), (place, b, t)
                     assert np.array_equal(np.delete(got[b, t], 3, -1), np.delete(clean[b, t], 3, -1)), (place, b, t)
                 else: assert np.array_equal(got[b, t], clean[b, t]), (place, b, t)
+
+
+@pytest.mark.parametrize("heads,lens,T,shared", [((16, 2, 256), [0, 5, 2, 0], 4, 0), ((6, 3, 64), [0, 200, 64, 1], 2, 128), ((16, 2, 256), [0, 900, 3], 24, 64), ((8, 1, 128), [0, 0], 1, 0)])
+def test_gates_of_rows_that_see_nothing(orn, ctx, heads, lens, T, shared):
+    """Padded rows are zeros whatever their queries and gates hold; the others do not notice."""
+    rng = np.random.default_rng(7)
+    Hq, Hkv, hd = heads
+    c = Case(ctx, rng, lens, T, shared, 64, Hq, Hkv, hd).upload(orn)
+    q, qg = util.bf16_normal(rng, (c.B, T, Hq, hd)), util.bf16_normal(rng, (c.B, T, Hq, 2 * hd))
+    clean = _attend(orn, ctx, c, q, qg, hd ** -0.5)
+    for b, n in enumerate(lens):
+        for t in range(T):
+            if n - T + t < 0:
+                assert not (clean[b, t] & 0x7fff).any()
+                q[b, t, :, ::3], qg[b, t, :, ::2], qg[b, t, :, 1::2] = 0x7f80, 0x7fc0, 0xff80
+    got = _attend(orn, ctx, c, q, qg, hd ** -0.5)
+    assert np.array_equal(got & 0x7fff, clean & 0x7fff) and np.array_equal(got[clean != 0], clean[clean != 0])
+    c.free()
