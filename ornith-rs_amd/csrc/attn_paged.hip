@@ -383,7 +383,7 @@ __device__ __forceinline__ void attend_part(const PagedArgs& p, int block, unsig
       // Pairs of probabilities: the next number below, cut to bf16, and what that leaves of each, rounded to bf16; a
       // product each, so that a probability counts to 2^-16 of itself. (Below, so that neither part of a probability
       // above zero is zero: times an infinite value that would be no number, where the result is infinite. The first part
-      // alone, 2^-8: 201 us for 222 at 2048 rows behind 32768 keys, 41.4 for 44.6 at 512 rows behind 16256, 1 %
+      // alone, 2^-8: 201 us for 215 at 2048 rows behind 32768 keys, 41.4 for 44.6 at 512 rows behind 16256, 1 %
       // where rows are few; the result's error against 64 bits was 2.2e-3 where its own rounding to bf16 makes 1.66e-3.)
       uint32_t pb[2][BK / 8];
 #pragma unroll
